@@ -196,9 +196,9 @@ def _plain_route(logits, bias, c):
         s = 1.0 / (1.0 + torch.exp(-x))
         part = s / (s.sum(-1, keepdim=True) + _TINY)
     pick = s.detach() if bias is None else s.detach() + bias
-    if c["score"] == "softmax" and bias is None and n == 1:
-        pick = x.detach()
-    if n > 1:
+    if bias is None and m == n:
+        pick = x.detach()  # the scores' own order, also where they round to the same value
+    if n > m:
         best = torch.sort(pick.view(t, n, e // n), dim=-1, descending=True).values[..., :max(1, k // m)]
         total = best.sum(-1)
         order = torch.sort(total, dim=-1, descending=True, stable=True).indices[:, :m]
@@ -350,7 +350,7 @@ def _exact_route(st):
     k, n, m = c["k"], c["groups"], c["top_groups"]
     s = torch.softmax(x, -1) if c["score"] == "softmax" else torch.sigmoid(x)
     pick = s + (st["bias"].double() if st["bias"] is not None else 0.0)
-    if n > 1:
+    if n > m:
         of = pick.view(t, n, -1).topk(max(1, k // m), -1).values.sum(-1)
         gone = torch.ones_like(of, dtype=torch.bool).scatter(1, of.argsort(dim=-1, descending=True, stable=True)[:, :m], False)
         pick = pick.masked_fill(gone[:, :, None].expand(t, n, e // n).reshape(t, e), -math.inf)
