@@ -21,6 +21,12 @@ std::vector<torch::Tensor> add_rmsnorm_fwd(torch::Tensor x, torch::Tensor o, tor
 torch::Tensor swiglu_fwd(torch::Tensor h);
 torch::Tensor swiglu_bwd(torch::Tensor dy, torch::Tensor h);
 torch::Tensor rope_fwd(torch::Tensor qkv, torch::Tensor cosv, torch::Tensor sinv, int64_t nrot, bool inverse);
+torch::Tensor heads_fwd(torch::Tensor qkv, torch::Tensor cosv, torch::Tensor sinv, int64_t nq, int64_t nk,
+                        bool interleaved, c10::optional<torch::Tensor> wq, c10::optional<torch::Tensor> wk, double eps);
+std::vector<torch::Tensor> heads_bwd(torch::Tensor dy, c10::optional<torch::Tensor> qkv, torch::Tensor cosv,
+                                     torch::Tensor sinv, int64_t nq, int64_t nk, bool interleaved,
+                                     c10::optional<torch::Tensor> wq, c10::optional<torch::Tensor> wk, double eps,
+                                     c10::optional<torch::Tensor> dwq_accum, c10::optional<torch::Tensor> dwk_accum);
 torch::Tensor ce_local_max(torch::Tensor logits);
 torch::Tensor ce_local_stats(torch::Tensor logits, torch::Tensor labels, torch::Tensor lmax, int64_t vstart);
 torch::Tensor ce_bwd(torch::Tensor logits, torch::Tensor labels, torch::Tensor lmax, torch::Tensor sumexp,
@@ -67,6 +73,11 @@ void gemm_grouped_wgrad(torch::Tensor dy, torch::Tensor x, torch::Tensor seg, to
 std::vector<torch::Tensor> moe_router_fwd(torch::Tensor logits, int64_t k);
 torch::Tensor moe_router_bwd(torch::Tensor logits, torch::Tensor top_idx, torch::Tensor probs, torch::Tensor dprobs,
                              torch::Tensor g_aux);
+std::vector<torch::Tensor> moe_route_fwd(torch::Tensor logits, int64_t k, bool sigmoid,
+                                         c10::optional<torch::Tensor> bias, int64_t groups, int64_t topg, bool renorm,
+                                         double scaling);
+torch::Tensor moe_route_bwd(torch::Tensor logits, torch::Tensor experts, c10::optional<torch::Tensor> dweights,
+                            c10::optional<torch::Tensor> dscore, bool sigmoid, bool renorm, double scaling);
 std::vector<torch::Tensor> moe_layout(torch::Tensor gid, torch::Tensor counts, int64_t rows_cap, int64_t align);
 torch::Tensor moe_scatter(torch::Tensor src, int64_t k_div, torch::Tensor pos, c10::optional<torch::Tensor> w,
                           torch::Tensor seg, torch::Tensor counts, int64_t rows_cap);
@@ -104,6 +115,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu_fwd", &swiglu_fwd);
   m.def("swiglu_bwd", &swiglu_bwd);
   m.def("rope_fwd", &rope_fwd);
+  m.def("heads_fwd", &heads_fwd);
+  m.def("heads_bwd", &heads_bwd);
   m.def("ce_local_max", &ce_local_max);
   m.def("ce_local_stats", &ce_local_stats);
   m.def("ce_bwd", &ce_bwd);
@@ -150,6 +163,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_grouped_wgrad", &gemm_grouped_wgrad);
   m.def("moe_router_fwd", &moe_router_fwd);
   m.def("moe_router_bwd", &moe_router_bwd);
+  m.def("moe_route_fwd", &moe_route_fwd);
+  m.def("moe_route_bwd", &moe_route_bwd);
   m.def("moe_layout", &moe_layout, py::arg("gid"), py::arg("counts"), py::arg("rows_cap"), py::arg("align") = 128);
   m.def("moe_scatter", &moe_scatter, py::arg("src"), py::arg("k_div"), py::arg("pos"), py::arg("w"), py::arg("seg"),
         py::arg("counts"), py::arg("rows_cap"));

@@ -15,6 +15,45 @@ from dataclasses import dataclass, field
 from typing import Optional
 
 
+@dataclass(frozen=True)
+class RopeScaling:
+    """How rotary frequencies are stretched to contexts longer than the ``original_max_position`` of pre-training."""
+
+    kind: str = "linear"  # "linear" | "llama3" | "yarn"
+    factor: float = 1.0
+    original_max_position: int = 8192
+    low_freq_factor: float = 1.0  # llama3: wavelengths over original / low are divided by the factor,
+    high_freq_factor: float = 4.0  # those under original / high are kept, in between both are mixed
+    beta_fast: float = 32.0  # yarn: channels with more turns than this over the original context are kept,
+    beta_slow: float = 1.0  # those with fewer than this are divided by the factor
+
+    def __post_init__(self):
+        if self.kind not in ("linear", "llama3", "yarn"):
+            raise ValueError(f"rope scaling must be linear, llama3 or yarn, got {self.kind!r}")
+        if self.factor < 1.0:
+            raise ValueError(f"the rope scaling factor must be at least 1, got {self.factor}")
+        if self.high_freq_factor <= self.low_freq_factor or self.beta_fast <= self.beta_slow:
+            raise ValueError("rope scaling bounds must be in order (low < high, beta_slow < beta_fast)")
+
+    def apply(self, inv_freq, dim: int, base: float):
+        """(scaled frequencies, factor of the tables) for the 64-bit frequencies of ``dim`` turned channels."""
+        slow = inv_freq / self.factor
+        if self.kind == "linear":
+            return slow, 1.0
+        turns = self.original_max_position * inv_freq / (2 * math.pi)  # over the original context
+        if self.kind == "llama3":
+            keep = ((turns - self.low_freq_factor) / (self.high_freq_factor - self.low_freq_factor)).clamp(0.0, 1.0)
+            return slow + (inv_freq - slow) * keep, 1.0
+
+        def channel(n):  # index of the frequency that turns n times over the original context
+            return dim * math.log(self.original_max_position / (n * 2 * math.pi)) / (2 * math.log(base))
+
+        lo = max(math.floor(channel(self.beta_fast)), 0)
+        hi = max(min(math.ceil(channel(self.beta_slow)), dim - 1), lo + 1e-3)
+        ramp = ((inv_freq.new_tensor(range(dim // 2)) - lo) / (hi - lo)).clamp(0.0, 1.0)
+        return slow * ramp + inv_freq * (1 - ramp), 0.1 * math.log(self.factor) + 1.0
+
+
 @dataclass
 class ModelConfig:
     """Architecture of a Llama-style GPT (dense or Mixtral-style MoE)."""

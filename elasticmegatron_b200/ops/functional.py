@@ -381,8 +381,101 @@ class RoPEFn(torch.autograd.Function):
         return out, None, None, None
 
 
-def rope_qkv(qkv, cos, sin, nrot):
-    return RoPEFn.apply(qkv, cos, sin, nrot)
+class HeadsFn(torch.autograd.Function):
+    """Rotary positions (any layout, part of the head, tables per sequence) of the first ``nq + nk`` slots of each
+    group of the fused qkv activations, with an RMSNorm of every such head before the turn where weights are given
+    (``csrc/ops/heads.cu``).  The backward re-reads qkv for the norm; without a norm it needs dy alone."""
+
+    @staticmethod
+    def forward(ctx, qkv, wq, wk, cos, sin, nq, nk, eps, interleaved):
+        ctx.save_for_backward(qkv if wq is not None else None, wq, wk, cos, sin)
+        ctx.rest = (nq, nk, interleaved)
+        ctx.eps = eps
+        if use_native(qkv):
+            return ext().heads_fwd(qkv, cos, sin, nq, nk, interleaved, wq, wk, eps)
+        return ref.heads_fwd(qkv, cos, sin, nq, nk, interleaved, wq, wk, eps)
+
+    @staticmethod
+    def backward(ctx, dy):
+        qkv, wq, wk, cos, sin = ctx.saved_tensors
+        nq, nk, interleaved = ctx.rest
+        none = (None,) * 6
+        mq, mk = getattr(wq, "main_grad", None), getattr(wk, "main_grad", None)
+        if use_native(dy):
+            out = ext().heads_bwd(dy, qkv, cos, sin, nq, nk, interleaved, wq, wk, ctx.eps,
+                                  mq.view(-1) if mq is not None else None, mk.view(-1) if mk is not None else None)
+            if wq is None:
+                return (out[0], None, None) + none
+            dx, dwq, dwk = out
+        else:
+            dx, dwq, dwk = ref.heads_bwd(dy, qkv, cos, sin, nq, nk, interleaved, wq, wk, ctx.eps)
+            if wq is None:
+                return (dx, None, None) + none
+            for m, g in ((mq, dwq), (mk, dwk)):
+                if m is not None:
+                    m.view(-1).add_(g)
+            dwq, dwk = dwq.to(wq.dtype), dwk.to(wk.dtype)
+        for w, m in ((wq, mq), (wk, mk)):
+            if m is not None and getattr(w, "_grad_ready", None) is not None:
+                w._grad_ready()
+        return (dx, dwq if mq is None else None, dwk if mk is None else None) + none
+
+
+def _check_heads(qkv, cos, sin, n):
+    if qkv.dim() != 5:
+        raise ValueError(f"qkv must be [s, b, groups, slots, d], got {tuple(qkv.shape)}")
+    s, b, _, slots, d = qkv.shape
+    if not 0 <= n <= slots:
+        raise ValueError(f"{n} turned heads do not fit the {slots} slots of a group")
+    if cos.shape != sin.shape or cos.dim() not in (2, 3) or tuple(cos.shape[:-1]) not in ((s,), (s, b)):
+        raise ValueError(f"cos and sin must both be [{s}, r/2] or [{s}, {b}, r/2], got {tuple(cos.shape)} and "
+                         f"{tuple(sin.shape)}")
+    if d % 2 or d > 512 or 2 * cos.shape[-1] > d:
+        raise ValueError(f"the head size must be even, at most 512 and hold the turned channels: d={d}, "
+                         f"r={2 * cos.shape[-1]}")
+
+
+def rope_qkv(qkv, cos, sin, nrot, interleaved: bool = False):
+    """Rotary positions of the first ``nrot`` slots (query heads and the key head) of each group of the fused
+    activations ``qkv`` [s, b, G, slots, d]; the other slots pass through.
+
+    ``cos`` / ``sin`` are fp32 [s, r/2], or [s, b, r/2] where the sequences of the batch have positions of their own
+    (:func:`rope_tables` makes them); the first ``r <= d`` channels of a head turn, in the pairs (i, i + r/2) or, with
+    ``interleaved``, (2i, 2i + 1).  bf16, fp16 or fp32; the result has the type of ``qkv``."""
+    _check_heads(qkv, cos, sin, nrot)
+    if not interleaved and cos.dim() == 2 and 2 * cos.shape[-1] == qkv.shape[-1] and qkv.dtype == torch.bfloat16:
+        return RoPEFn.apply(qkv, cos, sin, nrot)
+    return HeadsFn.apply(qkv, None, None, cos, sin, nrot, 0, 0.0, interleaved)
+
+
+def qk_norm_rope_qkv(qkv, q_weight, k_weight, cos, sin, eps, interleaved: bool = False):
+    """RMSNorm of every query and key head and their rotary positions in one pass over the fused activations
+    ``qkv`` [s, b, G, hpg + 2, d] (query heads, key head, value head of each group; values pass through).
+
+    ``q_weight`` / ``k_weight`` [d] have the type of ``qkv`` and are shared by all heads; their gradients accumulate
+    in fp32 into ``main_grad`` where the parameters have one.  Tables and layouts as for :func:`rope_qkv`."""
+    if qkv.dim() == 5 and qkv.shape[3] < 3:
+        raise ValueError("a group needs at least one query head, the key head and the value head")
+    _check_heads(qkv, cos, sin, qkv.shape[3] - 1 if qkv.dim() == 5 else 0)
+    for n, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if tuple(w.shape) != (qkv.shape[-1],) or w.dtype != qkv.dtype:
+            raise ValueError(f"{n} must be [{qkv.shape[-1]}] of qkv's type {qkv.dtype}, got {tuple(w.shape)} {w.dtype}")
+    return HeadsFn.apply(qkv, q_weight, k_weight, cos, sin, qkv.shape[3] - 2, 1, eps, interleaved)
+
+
+def rope_tables(positions: torch.Tensor, dim: int, base: float, scaling=None):
+    """fp32 (cos, sin) of shape ``positions.shape + (dim/2,)`` for ``dim`` turned channels, from 64-bit angles.
+
+    ``scaling`` (:class:`~elasticmegatron_b200.config.RopeScaling`) stretches the positions to a longer context than the
+    model was trained on: ``linear`` divides all of them by the factor, ``llama3`` only those of the wavelengths that
+    do not fit the original context, ``yarn`` ramps between the two by the number of turns and also scales the tables
+    (the attention temperature; the backward of the rotation is its transpose, so the factor carries over)."""
+    inv = 1.0 / (base ** (torch.arange(0, dim, 2, dtype=torch.float64, device=positions.device) / dim))
+    amp = 1.0
+    if scaling is not None:
+        inv, amp = scaling.apply(inv, dim, base)
+    ang = positions.to(torch.float64)[..., None] * inv
+    return (amp * ang.cos()).float(), (amp * ang.sin()).float()
 
 
 # ------------------------------------------------------------------------------------------ attention
@@ -457,6 +550,58 @@ def attention(qkv, hpg):
     if qkv.is_cuda and not (_has_native_attention() and ext().attn_supported(qkv)):
         return _sdpa_attention(qkv, hpg)
     return AttentionFn.apply(qkv, hpg)
+
+
+# ------------------------------------------------------------------------------------------ MoE router
+class MoERouteFn(torch.autograd.Function):
+    """(weights [T, k], score_sum [E], experts [T, k], counts [E]) of :func:`moe_route`."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, k, sigmoid, groups, topg, renorm, scaling):
+        fwd = ext().moe_route_fwd if use_native(logits) else ref.moe_route_fwd
+        weights, experts, score_sum, counts = fwd(logits, k, sigmoid, bias, groups, topg, renorm, scaling)
+        ctx.save_for_backward(logits, experts)
+        ctx.rest = (sigmoid, renorm, scaling)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(experts, counts)
+        return weights, score_sum, experts, counts
+
+    @staticmethod
+    def backward(ctx, dweights, dscore, _experts, _counts):
+        logits, experts = ctx.saved_tensors
+        bwd = ext().moe_route_bwd if use_native(logits) else ref.moe_route_bwd
+        return (bwd(logits, experts, dweights, dscore, *ctx.rest),) + (None,) * 7
+
+
+def moe_route(logits, k: int, score_function: str = "softmax", bias: Optional[torch.Tensor] = None, num_groups: int = 1,
+              group_topk: int = 1, renormalize: bool = False, scaling: float = 1.0):
+    """Routes tokens to ``k`` of E experts by ``logits`` [T, E]; returns ``(weights, experts, score_sum, counts)``.
+
+    Scores are ``softmax`` or ``sigmoid`` of the logits (fp32).  ``bias`` [E] (fp32) is added for the selection only, as
+    balancing without an auxiliary loss does.  With ``num_groups`` > 1 the experts of the ``group_topk`` best groups of
+    neighbours compete; a group's value is the sum of its ``max(1, k // group_topk)`` best.  Ties go to the lower
+    index, and a logit of -inf masks an expert: it comes after every other expert of the kept groups and weighs 0.
+
+    ``weights`` [T, k] fp32 are the chosen scores in falling order of choice, divided by their sum with ``renormalize``,
+    times ``scaling``; ``experts`` [T, k] int32; ``score_sum`` [E] is the sum over the tokens of the scores (sigmoid
+    scores normalised over the experts) for a load-balancing loss; ``counts`` [E] int32 the tokens of each expert.
+    ``weights`` and ``score_sum`` carry gradients to ``logits``."""
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [tokens, experts], got {tuple(logits.shape)}")
+    E = logits.shape[1]
+    if score_function not in ("softmax", "sigmoid"):
+        raise ValueError(f"score_function must be softmax or sigmoid, got {score_function!r}")
+    if not (1 <= E <= 512 and 1 <= k <= min(E, 32)):
+        raise ValueError(f"1 to 512 experts and 1 <= k <= min(experts, 32) are supported, got {E} and k={k}")
+    if not (1 <= num_groups <= 32) or E % num_groups:
+        raise ValueError(f"{E} experts do not divide into {num_groups} groups (at most 32)")
+    if not (1 <= group_topk <= num_groups) or group_topk * (E // num_groups) < k:
+        raise ValueError(f"{group_topk} of {num_groups} groups of {E // num_groups} do not hold k={k} experts")
+    if bias is not None and (tuple(bias.shape) != (E,) or bias.dtype != torch.float32):
+        raise ValueError(f"bias must be fp32 [{E}], got {tuple(bias.shape)} {bias.dtype}")
+    weights, score_sum, experts, counts = MoERouteFn.apply(logits, bias, k, score_function == "sigmoid", num_groups,
+                                                           group_topk, renormalize, scaling)
+    return weights, experts, score_sum, counts
 
 
 # ------------------------------------------------------------------------------------------ vocab-parallel CE

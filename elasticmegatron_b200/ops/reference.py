@@ -97,3 +97,116 @@ def adam_step(master, exp_avg, exp_avg_sq, grad, lr, beta1, beta2, eps, wd, step
     if wd != 0.0:
         master.mul_(1 - lr * wd)
     master.addcdiv_(exp_avg, denom, value=-lr / bc1)
+
+
+# ------------------------------------------------------------------------------------------ rotary positions
+def rope_rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool = False,
+                inverse: bool = False) -> torch.Tensor:
+    """Turns the first ``r = 2 * cos.shape[-1]`` channels of x [s, b, ..., d] (fp32 result); the tables are
+    [s, r/2] or [s, b, r/2] and the pairs (i, i + r/2) or, interleaved, (2i, 2i + 1)."""
+    h = cos.shape[-1]
+    shape = (x.shape[0], cos.shape[1] if cos.dim() == 3 else 1) + (1,) * (x.dim() - 3) + (h,)
+    c, s = cos.reshape(shape), sin.reshape(shape)
+    if inverse:
+        s = -s
+    xf = x.float()
+    y = xf.clone()
+    a, b = (slice(0, 2 * h, 2), slice(1, 2 * h, 2)) if interleaved else (slice(0, h), slice(h, 2 * h))
+    y[..., a] = xf[..., a] * c - xf[..., b] * s
+    y[..., b] = xf[..., b] * c + xf[..., a] * s
+    return y
+
+
+def heads_fwd(qkv, cos, sin, nq, nk, interleaved, wq=None, wk=None, eps=0.0) -> torch.Tensor:
+    """Rotary positions of the first nq + nk slots of each group of qkv [s, b, G, S, d], after an RMSNorm of every
+    head where weights are given."""
+    y = qkv.float().clone()
+    n = nq + nk
+    if wq is not None:
+        x = y[:, :, :, :n]
+        w = torch.cat([wq.float().expand(nq, -1), wk.float().expand(nk, -1)])
+        y[:, :, :, :n] = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * w
+    y[:, :, :, :n] = rope_rotate(y[:, :, :, :n], cos, sin, interleaved)
+    return y.to(qkv.dtype)
+
+
+def heads_bwd(dy, qkv, cos, sin, nq, nk, interleaved, wq=None, wk=None, eps=0.0):
+    """(dqkv, dwq, dwk) of :func:`heads_fwd`; the weight gradients are fp32 (None without norm)."""
+    n = nq + nk
+    dx = dy.float().clone()
+    g = rope_rotate(dx[:, :, :, :n], cos, sin, interleaved, inverse=True)
+    if wq is None:
+        dx[:, :, :, :n] = g
+        return dx.to(dy.dtype), None, None
+    x = qkv[:, :, :, :n].float()
+    rstd = torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps)
+    xh = x * rstd
+    dw = (g * xh).sum((0, 1, 2))
+    gw = g * torch.cat([wq.float().expand(nq, -1), wk.float().expand(nk, -1)])
+    dx[:, :, :, :n] = rstd * (gw - xh * (gw * xh).mean(-1, keepdim=True))
+    return dx.to(dy.dtype), dw[:nq].sum(0), dw[nq:].sum(0)
+
+
+# ------------------------------------------------------------------------------------------ router
+_TINY = 1e-20
+
+
+def _route_scores(x, sigmoid):
+    """(scores, what the normalised scores of the statistics are divided by)."""
+    if sigmoid:
+        s = 1.0 / (1.0 + torch.exp(-x))
+        return s, s.sum(-1, keepdim=True) + _TINY
+    m = x.max(-1, keepdim=True).values
+    e = torch.where(x == -math.inf, torch.zeros_like(x), torch.exp(x - m))
+    # the sum is held in 64 bits so that the choice does not depend on the order of the additions
+    z = e.double().sum(-1, keepdim=True).float()
+    return e / torch.where(z == 0, torch.ones_like(z), z), torch.ones_like(z)
+
+
+def moe_route_fwd(logits, k, sigmoid, bias, groups, topg, renorm, scaling):
+    """(weights [T, k], experts [T, k] int32, score_sum [E], counts [E] int32); see ``csrc/moe/route.cu``."""
+    x = logits.float()
+    T, E = x.shape
+    s, norm = _route_scores(x, sigmoid)
+    c = s if bias is None else s + bias
+    if bias is None and topg == groups:
+        c = x  # the scores' own order, also where they round to the same value
+    # masked and NaN entries come after every other expert, experts of dropped groups after those
+    c = torch.where((x > -math.inf) & ~c.isnan(), c, torch.full_like(c, -math.inf))
+    lost = torch.zeros(T, E, dtype=torch.bool, device=x.device)
+    if groups > topg:
+        best = c.view(T, groups, E // groups).sort(-1, descending=True).values
+        best = best[..., :min(max(1, k // topg), E // groups)]
+        value = torch.where(best == -math.inf, torch.zeros_like(best), best).sum(-1)
+        value = torch.where(best[..., 0] == -math.inf, best[..., 0], value)
+        order = value.sort(dim=-1, descending=True, stable=True).indices[:, :topg]
+        lost = torch.ones_like(value, dtype=torch.bool).scatter(1, order, False).repeat_interleave(E // groups, 1)
+    order = c.sort(dim=-1, descending=True, stable=True).indices
+    kept = (~lost).gather(1, order)  # in order, the experts of dropped groups moved to the end
+    order = order.gather(1, kept.to(torch.int8).sort(dim=-1, descending=True, stable=True).indices)
+    top = order[:, :k]
+    w = s.gather(1, top)
+    if renorm:
+        w = w / (w.sum(-1, keepdim=True) + _TINY)
+    counts = torch.bincount(top.reshape(-1), minlength=E).to(torch.int32)
+    return w * scaling, top.to(torch.int32), (s / norm).sum(0), counts
+
+
+def moe_route_bwd(logits, experts, dweights, dscore, sigmoid, renorm, scaling):
+    x = logits.float()
+    s, norm = _route_scores(x, sigmoid)
+    top = experts.long()
+    u = s.gather(1, top)
+    a = dweights.float() * scaling if dweights is not None else torch.zeros_like(u)
+    if renorm:
+        den = u.sum(-1, keepdim=True) + _TINY
+        a = (a - (a * u / den).sum(-1, keepdim=True)) / den
+    ds = torch.zeros_like(s).scatter(1, top, a)
+    q = dscore.float()[None] if dscore is not None else torch.zeros(1, x.shape[1], device=x.device)
+    if sigmoid:
+        e = torch.exp(-x.abs())
+        dl = e / (1 + e) ** 2 * (ds + (q - (q * s).sum(-1, keepdim=True) / norm) / norm)
+    else:
+        g = ds + q
+        dl = s * (g - (s * g).sum(-1, keepdim=True))
+    return dl.to(logits.dtype)
