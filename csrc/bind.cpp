@@ -31,6 +31,11 @@ torch::Tensor ce_local_max(torch::Tensor logits);
 torch::Tensor ce_local_stats(torch::Tensor logits, torch::Tensor labels, torch::Tensor lmax, int64_t vstart);
 torch::Tensor ce_bwd(torch::Tensor logits, torch::Tensor labels, torch::Tensor lmax, torch::Tensor sumexp,
                      torch::Tensor dloss, int64_t vstart);
+std::vector<torch::Tensor> linear_ce_fwd(torch::Tensor x, torch::Tensor w, torch::Tensor labels, int64_t col0,
+                                         int64_t vocab, int64_t ignore, bool raw);
+std::vector<torch::Tensor> linear_ce_bwd(torch::Tensor dloss, torch::Tensor x, torch::Tensor w, torch::Tensor labels,
+                                         torch::Tensor top, torch::Tensor sum, int64_t col0, int64_t vocab, int64_t ignore, bool want_dx,
+                                         bool want_dw, c10::optional<torch::Tensor> dw_accum, int64_t piece);
 torch::Tensor embedding_fwd(torch::Tensor ids, torch::Tensor w, int64_t vstart);
 void embedding_bwd(torch::Tensor ids, torch::Tensor dy, torch::Tensor target, int64_t vstart);
 void adam_segments(torch::Tensor O, torch::Tensor G, torch::Tensor P, torch::Tensor chunks, double lr, double b1,
@@ -120,6 +125,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_local_max", &ce_local_max);
   m.def("ce_local_stats", &ce_local_stats);
   m.def("ce_bwd", &ce_bwd);
+  m.def("linear_ce_fwd", &linear_ce_fwd);
+  m.def("linear_ce_bwd", &linear_ce_bwd);
   m.def("embedding_fwd", &embedding_fwd);
   m.def("embedding_bwd", &embedding_bwd);
   m.def("adam_segments", &adam_segments, py::arg("O"), py::arg("G"), py::arg("P"), py::arg("chunks"), py::arg("lr"),

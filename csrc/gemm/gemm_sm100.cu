@@ -27,6 +27,7 @@
 #include <atomic>
 
 #include "../include/common.cuh"
+#include "linear_ce.cuh"
 
 namespace emb {
 namespace gk {
@@ -164,6 +165,8 @@ struct Params {
   // group_info[m tile] = group of that tile (-1: skip); B holds every group's matrix stacked along its row
   // coordinate, group g's rows start at g * group_b_stride.  group_mode 2 (weight gradient): group g reduces
   // over rows [group_info[g], group_info[g + 1]) of A and B (multiples of BK) into C + g * group_c_stride.
+  // group_mode 3 (one product split along K): group g takes the g-th of `groups` equal shares of the k-blocks into
+  // C + g * group_c_stride.
   int group_mode;
   const int* group_info;
   int groups;
@@ -191,7 +194,12 @@ struct Params {
   int ag_tp;
   int ag_units_max;
   uint32_t ag_epoch;
+  CeArgs ce;  // cross-entropy epilogues (EPI 1 and 2) only
 };
+
+// What the epilogue does with an accumulator: stores it; keeps a row's maximum and sum of exponentials over the tile
+// (and its label's logit); or turns it into the gradient of the logits before the store.
+enum Epilogue { kStore = 0, kCeStats = 1, kCeGrad = 2 };
 
 struct TileInfo {
   int m0, n0, kb0, kb1, b_off;
@@ -212,6 +220,17 @@ __device__ __forceinline__ bool tile_info(const Params& p, int t, int tiles_m, i
     ti.c_off = (long long)g * p.group_c_stride;
     return ti.kb1 > ti.kb0;
   }
+  if (p.group_mode == 3) {
+    const int per = tiles_m * tiles_n;
+    const int g = t / per, r = t - g * per;
+    ti.m0 = (r % tiles_m) * BM;
+    ti.n0 = (r / tiles_m) * BN;
+    ti.kb0 = (int)((long long)nk * g / p.groups);
+    ti.kb1 = (int)((long long)nk * (g + 1) / p.groups);
+    ti.b_off = 0;
+    ti.c_off = (long long)g * p.group_c_stride;
+    return true;
+  }
   if (p.group_mode == 0 && tiles_n < tiles_m && !p.m_fast) {
     ti.m0 = (t / tiles_n) * BM;
     ti.n0 = (t % tiles_n) * BN;
@@ -231,6 +250,7 @@ __device__ __forceinline__ bool tile_info(const Params& p, int t, int tiles_m, i
   return true;
 }
 
+template <int EPI>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -248,7 +268,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const int lane = threadIdx.x & 31;
   const int tiles_m = (p.M + BM - 1) / BM;
   const int tiles_n = (p.N + BN - 1) / BN;
-  const int num_tiles = tiles_m * tiles_n * (p.group_mode == 2 ? p.groups : 1);
+  const int num_tiles = tiles_m * tiles_n * (p.group_mode >= 2 ? p.groups : 1);
   const int nk = (p.K + BK - 1) / BK;
 
   if (threadIdx.x == 0) {
@@ -360,6 +380,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int n0 = ti.n0;
       const int row = m0 + row_in_tile;
       const bool row_ok = row < p.M;
+      if constexpr (EPI == kCeStats) {
+        ce_stats_tile(p.ce, tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * BN, n0, p.N, row, p.M, n0 / BN);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[buf]);
+        continue;
+      }
+      CeRow ce_row;
+      if constexpr (EPI == kCeGrad) ce_row = ce_load_row(p.ce, row, p.M);
 #pragma unroll 1
       for (int c = 0; c < BN / 32; ++c) {
         uint32_t r[32];
@@ -369,6 +398,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int col0 = n0 + c * 32;
         if (!row_ok || col0 >= p.N) continue;
         const int ncols = min(32, p.N - col0);
+        if constexpr (EPI == kCeGrad) ce_grad_chunk(ce_row, r, col0);
         if (p.out_fp32) {
           float* dst = reinterpret_cast<float*>(p.C) + ti.c_off + (size_t)row * p.ldc + col0;
           if (ncols == 32 && ((reinterpret_cast<uintptr_t>(dst) & 15) == 0)) {
@@ -531,7 +561,7 @@ __device__ __forceinline__ bool wait_epoch(const uint32_t* flag, uint32_t epoch,
   return false;
 }
 
-template <bool AG, int BK_>
+template <bool AG, int BK_, int EPI>
 __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
     gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmC, gk::Params p) {
@@ -783,6 +813,15 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
       const int n0 = tile_n(t) * BN + (hf > 0 ? BN / 2 : 0);
       const int n_chunks = (hf >= 0 ? BN / 2 : BN) / 32;
       const bool row_ok = row < p.M;
+      if constexpr (EPI == kCeStats) {
+        ce_stats_tile(p.ce, tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * BN, n0, p.N, row, p.M, n0 / BN);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) remote_arrive(mapa(smem_u32(&tempty[buf]), 0));
+        continue;
+      }
+      CeRow ce_row;
+      if constexpr (EPI == kCeGrad) ce_row = ce_load_row(p.ce, row, p.M);
       if (p.c_tma && !p.no_store) {
         // Each warp stages its 32 rows x 128 bytes (32 fp32 or 64 bf16 columns) in a 128-byte-swizzled block
         // (16-byte chunk j of row r at chunk j ^ (r & 7): conflict-free writes) and one lane hands the block to
@@ -799,6 +838,10 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
           TMEM_LD_32(taddr, r);
           if (!p.out_fp32) TMEM_LD_32(taddr + 32, (r + 32));
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          if constexpr (EPI == kCeGrad) {
+            ce_grad_chunk(ce_row, r, n0 + c * cols);
+            ce_grad_chunk(ce_row, r + 32, n0 + c * cols + 32);
+          }
           uint8_t* wbuf = sEpi + (epi_n & 1) * 16384 + quarter * 4096;
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
           __syncwarp();
@@ -850,6 +893,7 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
         const int col0 = n0 + c * 32;
         if (!row_ok || col0 >= p.N || p.no_store) continue;
         const int ncols = min(32, p.N - col0);
+        if constexpr (EPI == kCeGrad) ce_grad_chunk(ce_row, r, col0);
         void* gdst;
         if (p.scatter) {
           // fused reduce-scatter: this partial row chunk goes straight to its owner's staging slot (peer memory
@@ -981,6 +1025,15 @@ static PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
     TORCH_CHECK(q == cudaDriverEntryPointSuccess && p, "cuTensorMapEncodeTiled not available");
     fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
   }
+  // The encoder is a driver call and needs a current context.  A thread that has made no runtime call yet has none
+  // (autograd's worker when a product is the first thing it runs): selecting the device makes its context current.
+  static thread_local int ready_dev = -1;
+  int dev = 0;
+  EMB_CUDA_CHECK(cudaGetDevice(&dev));
+  if (ready_dev != dev) {
+    EMB_CUDA_CHECK(cudaSetDevice(dev));
+    ready_dev = dev;
+  }
   return fn;
 }
 
@@ -996,6 +1049,23 @@ static CUtensorMap make_map(const void* base, int64_t rows, int64_t cols, int64_
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed: ", (int)r);
   return m;
+}
+
+// Tensor map of an output [M, N] with 16-byte aligned rows (false otherwise): 32-row boxes of 128 bytes, 128-byte
+// swizzle.
+static bool make_c_map(const at::Tensor& C, bool fp32, int64_t M, int64_t N, CUtensorMap& m) {
+  const int esz = fp32 ? 4 : 2;
+  if (((uintptr_t)C.data_ptr() % 16) != 0 || (C.stride(0) * esz) % 16 != 0) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
+  cuuint64_t strides[1] = {(cuuint64_t)(C.stride(0) * esz)};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / esz), 32};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = get_encode()(&m, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                            C.data_ptr(), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled(C) failed: ", (int)r);
+  return true;
 }
 
 static int* err_flag() { return device_err_flag(kErrGemm); }
@@ -1031,14 +1101,14 @@ static int gemm2_default_bk() {
 namespace gk2 {
 // Launch the 2-SM kernel on `clusters` CTA pairs with stage depth `bk` (64 or 128); sets the kernel's
 // shared-memory limit on each device the first time it is used there.
-template <bool AG>
+template <bool AG, int EPI = gk::kStore>
 static void launch(int bk, const CUtensorMap& tA, const CUtensorMap& tB, const CUtensorMap& tC, const gk::Params& p,
                    int clusters) {
   static bool attr_set[2][kMaxDevices] = {};
   int dev = 0;
   EMB_CUDA_CHECK(cudaGetDevice(&dev));
   const int which = bk == 128 ? 1 : 0;
-  auto kern = which ? gemm2_kernel<AG, 128> : gemm2_kernel<AG, 64>;
+  auto kern = which ? gemm2_kernel<AG, 128, EPI> : gemm2_kernel<AG, 64, EPI>;
   const int smem = which ? smem_bytes<128>() : smem_bytes<64>();
   if (!attr_set[which][dev]) {
     EMB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -1066,12 +1136,13 @@ static bool ok_2d(const at::Tensor& t) {
 
 // The 1-SM kernel's dynamic shared-memory limit, raised once per device (a function attribute belongs to the
 // device's context).
+template <int EPI = gk::kStore>
 static void gemm1_smem_attr() {
   static bool done[kMaxDevices] = {};
   int dev = 0;
   EMB_CUDA_CHECK(cudaGetDevice(&dev));
   if (!done[dev]) {
-    EMB_CUDA_CHECK(cudaFuncSetAttribute(gk::gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gk::SMEM_BYTES));
+    EMB_CUDA_CHECK(cudaFuncSetAttribute(gk::gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, gk::SMEM_BYTES));
     done[dev] = true;
   }
 }
@@ -1144,28 +1215,16 @@ at::Tensor gemm_tc(at::Tensor a, at::Tensor b, bool trans_a, bool trans_b, c10::
     // 2-SM clusters: each CTA loads a 128-row half of the A tile and of the B tile
     CUtensorMap tA2 = a_mn ? make_map(a.data_ptr(), K, M, a.stride(0), 64, bk) : make_map(a.data_ptr(), M, K, a.stride(0), 64, 128);
     CUtensorMap tB2 = b_mn ? make_map(b.data_ptr(), K, N, b.stride(0), 64, bk) : make_map(b.data_ptr(), N, K, b.stride(0), 64, 128);
-    // C through a tensor map when its rows are 16-byte aligned: 32-row boxes of 128 bytes, 128-byte swizzle
+    // C through a tensor map when its rows are 16-byte aligned
     CUtensorMap tC = tA2;
-    const int esz = p.out_fp32 ? 4 : 2;
-    if (((uintptr_t)C.data_ptr() % 16) == 0 && (C.stride(0) * esz) % 16 == 0 && p.no_store == 0) {
-      cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
-      cuuint64_t strides[1] = {(cuuint64_t)(C.stride(0) * esz)};
-      cuuint32_t box[2] = {(cuuint32_t)(128 / esz), 32};
-      cuuint32_t estr[2] = {1, 1};
-      CUresult r = get_encode()(&tC, p.out_fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                                C.data_ptr(), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-      TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled(C) failed: ", (int)r);
-      p.c_tma = c_tma_enabled() ? 1 : 0;
-    }
+    if (p.no_store == 0 && make_c_map(C, p.out_fp32, M, N, tC)) p.c_tma = c_tma_enabled() ? 1 : 0;
     const int clusters = (int)std::min<int64_t>(tiles2, num_sms() / 2);
     gk2::launch<false>(bk, tA2, tB2, tC, p, clusters);
   } else {
     gemm1_smem_attr();
     const int tiles = (int)(((M + BM - 1) / BM) * ((N + BN - 1) / BN));
     const int grid = std::min(tiles, num_sms());
-    gemm_kernel<<<grid, NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
+    gemm_kernel<kStore><<<grid, NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
   }
   EMB_LAUNCH_CHECK();
   count_launch();
@@ -1206,7 +1265,7 @@ at::Tensor gemm_grouped(at::Tensor a, at::Tensor w, bool trans_b, at::Tensor til
   p.group_b_stride = (int)(trans_b ? N : K);
   gemm1_smem_attr();
   const int tiles = (int)((R / BM) * ((N + BN - 1) / BN));
-  gemm_kernel<<<std::min(tiles, num_sms()), NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
+  gemm_kernel<kStore><<<std::min(tiles, num_sms()), NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
   EMB_LAUNCH_CHECK();
   count_launch();
   return C;
@@ -1247,7 +1306,76 @@ void gemm_grouped_wgrad(at::Tensor dy, at::Tensor x, at::Tensor seg, at::Tensor 
   p.group_c_stride = (long long)M * N;
   gemm1_smem_attr();
   const int64_t tiles = G * ((M + BM - 1) / BM) * ((N + BN - 1) / BN);
-  gemm_kernel<<<(int)std::min<int64_t>(tiles, num_sms()), NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
+  gemm_kernel<kStore><<<(int)std::min<int64_t>(tiles, num_sms()), NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
+  EMB_LAUNCH_CHECK();
+  count_launch();
+}
+
+// Logits product of the linear cross entropy: x [T, H] @ w [V, H]^T with a cross-entropy epilogue.  `grad` false: row
+// statistics into ce.part / ce.target, nothing else is written.  `grad` true: the gradient of the logits in bf16 into
+// out [T, V] (row stride a multiple of 8).  Up to 128 rows run as 128-row tiles on single SMs: the product then reads w
+// at memory speed and a 256-row tile would do twice the tensor work for nothing.
+void linear_ce_gemm(const at::Tensor& x, const at::Tensor& w, const CeArgs& ce, bool grad, const at::Tensor& out) {
+  using namespace gk;
+  TORCH_CHECK(ok_2d(x) && ok_2d(w), "linear cross entropy: x and w need 16-byte aligned rows");
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  Params p{};
+  p.M = (int)M;
+  p.N = (int)N;
+  p.K = (int)K;
+  p.err = err_flag();
+  p.ce = ce;
+  if (grad) {
+    p.C = out.data_ptr();
+    p.ldc = (int)out.stride(0);
+  }
+  if (M > BM) {
+    CUtensorMap tA = make_map(x.data_ptr(), M, K, x.stride(0), 64, 128), tB = make_map(w.data_ptr(), N, K, w.stride(0), 64, 128);
+    CUtensorMap tC = tA;
+    p.split_tail = grad ? 1 : 0;  // the statistics have one slot for each whole tile
+    if (grad) p.c_tma = make_c_map(out, false, M, N, tC) ? 1 : 0;
+    const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
+    const int clusters = (int)std::min<int64_t>(tiles, num_sms() / 2);
+    if (grad) gk2::launch<false, kCeGrad>(128, tA, tB, tC, p, clusters);
+    else gk2::launch<false, kCeStats>(128, tA, tB, tC, p, clusters);
+  } else {
+    CUtensorMap tA = make_map(x.data_ptr(), M, K, x.stride(0), 64, BM), tB = make_map(w.data_ptr(), N, K, w.stride(0), 64, BN);
+    const int grid = (int)std::min<int64_t>((N + BN - 1) / BN, num_sms());
+    if (grad) {
+      gemm1_smem_attr<kCeGrad>();
+      gemm_kernel<kCeGrad><<<grid, NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
+    } else {
+      gemm1_smem_attr<kCeStats>();
+      gemm_kernel<kCeStats><<<grid, NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
+    }
+  }
+  EMB_LAUNCH_CHECK();
+  count_launch();
+}
+
+// parts[g] = a[:, share g of K] @ b[share g of K, :] in fp32 for equal shares of the 64-deep k-blocks (each has at
+// least one): a [M, K], b [K, N] bf16, parts [shares, M, N].  For products with few output tiles and a long K.
+void gemm_split_k(const at::Tensor& a, const at::Tensor& b, const at::Tensor& parts) {
+  using namespace gk;
+  TORCH_CHECK(ok_2d(a) && ok_2d(b) && parts.scalar_type() == at::kFloat && parts.is_contiguous(), "gemm_split_k: operands");
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
+  TORCH_CHECK(parts.size(0) >= 1 && parts.size(0) <= (K + BK - 1) / BK, "gemm_split_k: more shares than k-blocks");
+  CUtensorMap tA = make_map(a.data_ptr(), M, K, a.stride(0), 64, BM), tB = make_map(b.data_ptr(), K, N, b.stride(0), 64, 64);
+  Params p{};
+  p.C = parts.data_ptr();
+  p.M = (int)M;
+  p.N = (int)N;
+  p.K = (int)K;
+  p.ldc = (int)N;
+  p.out_fp32 = 1;
+  p.b_mn = 1;
+  p.err = err_flag();
+  p.group_mode = 3;
+  p.groups = (int)parts.size(0);
+  p.group_c_stride = (long long)M * N;
+  gemm1_smem_attr();
+  const int64_t tiles = p.groups * ((M + BM - 1) / BM) * ((N + BN - 1) / BN);
+  gemm_kernel<kStore><<<(int)std::min<int64_t>(tiles, num_sms()), NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
   EMB_LAUNCH_CHECK();
   count_launch();
 }

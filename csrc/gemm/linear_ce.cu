@@ -1,0 +1,197 @@
+// Linear cross entropy: loss_t = log sum_v exp(z_tv) - z_t,label(t) with z = x w^T, without keeping z [T, V].
+//
+// forward:  one product whose epilogue (linear_ce.cuh) leaves (max, sum exp) for each row and 256 columns, and the
+//           label's logit; a join over the column tiles.  2 T V H operations, and T V / 32 bytes of statistics in place
+//           of 2 T V of logits.
+// backward, per piece [v0, v1) of the vocabulary, with P = (softmax(z) - onehot) dloss of that piece only:
+//           product again with the gradient epilogue -> P (bf16);   dx += P w[v0:v1] (fp32);   dw[v0:v1] (+)= P^T x.
+//           6 T V H operations: 2 more than with kept logits.
+// P is rounded to bf16 because the tensor cores multiply bf16; everything summed over V or T is summed in fp32.
+#include "linear_ce.cuh"
+
+#include <c10/cuda/CUDAGuard.h>
+
+namespace emb {
+namespace {
+
+// Joins the tiles' statistics of a row: 32 rows a CTA, 32 slices of the tiles, in a fixed order.
+__global__ void __launch_bounds__(1024) ce_join_kernel(CeArgs ce, int T, int tiles, int V, bool raw,
+                                                       float* __restrict__ out, float* __restrict__ out_top,
+                                                       float* __restrict__ out_sum) {
+  __shared__ float sm[32][33], ss[32][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
+  float m = -INFINITY, s = 0.f;
+  if (row < T) {
+    for (int i = slice; i < tiles; i += 32) {
+      const float2 v = ce.part[(size_t)i * T + row];
+      const float top = fmaxf(m, v.x), base = top == -INFINITY ? 0.f : top;
+      s = s * __expf(m - base) + v.y * __expf(v.x - base);
+      m = top;
+    }
+  }
+  sm[slice][lane] = m;
+  ss[slice][lane] = s;
+  __syncthreads();
+  m = sm[lane][slice];  // slices of row blockIdx.x * 32 + slice
+  s = ss[lane][slice];
+  const float top = warp_max(m), base = top == -INFINITY ? 0.f : top;
+  s = warp_sum(s * __expf(m - base));
+  const int t = blockIdx.x * 32 + slice;
+  if (lane != 0 || t >= T) return;
+  const int64_t label = ce.labels[t];
+  const bool counts = ce_counts(ce, label);
+  const bool own = counts && label >= ce.col0 && label < ce.col0 + V;
+  out_top[t] = top;
+  out_sum[t] = s;
+  // a rank's share of the vocabulary leaves the label's logit, for the caller to join the ranks
+  out[t] = !own ? 0.f : raw ? ce.target[t] : logf(s) + (top - ce.target[t]);
+}
+
+// out[i] = bf16(sum over the n fp32 parts, in order)
+__global__ void parts_sum_kernel(const float4* __restrict__ parts, int n, int64_t vecs, __nv_bfloat16* __restrict__ out) {
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < vecs; i += (int64_t)gridDim.x * blockDim.x) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < n; ++p) {
+      const float4 v = parts[p * vecs + i];
+      a.x += v.x;
+      a.y += v.y;
+      a.z += v.z;
+      a.w += v.w;
+    }
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(a.x, a.y), __floats2bfloat162_rn(a.z, a.w)};
+    reinterpret_cast<uint2*>(out)[i] = *reinterpret_cast<uint2*>(h);
+  }
+}
+
+void check_ce(const at::Tensor& x, const at::Tensor& w, const at::Tensor& labels) {
+  TORCH_CHECK(x.is_cuda() && w.is_cuda() && labels.is_cuda() && x.device() == w.device() && x.device() == labels.device(),
+              "x, w and labels must be on one CUDA device");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16, "x and w must be bf16");
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && x.size(1) % 8 == 0 && x.size(1) > 0,
+              "x [T, H] and w [V, H] with H a multiple of 8");
+  TORCH_CHECK(labels.scalar_type() == at::kLong && labels.dim() == 1 && labels.size(0) == x.size(0) && labels.is_contiguous(),
+              "labels must be a contiguous int64 [T]");
+  TORCH_CHECK(x.size(0) < (1ll << 31) - 256 && w.size(0) < (1ll << 31) - 256, "too many rows");
+}
+
+// A 2-D operand that the tensor maps can take (16-byte rows), copied otherwise.
+at::Tensor tma_rows(const at::Tensor& t) {
+  const bool ok = t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) &&
+                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return ok ? t : at::empty(t.sizes(), t.options()).copy_(t);
+}
+
+CeArgs ce_args(const at::Tensor& labels, int64_t col0, int64_t vocab, int64_t ignore) {
+  CeArgs ce{};
+  ce.labels = labels.data_ptr<int64_t>();
+  ce.col0 = col0;
+  ce.vocab = vocab;
+  ce.ignore = ignore;
+  return ce;
+}
+
+// Columns of a piece of the vocabulary in the backward pass: as many as keep its bf16 gradient within 256 MiB.
+constexpr int64_t kPieceBytes = 256ll << 20;
+
+}  // namespace
+
+// {loss [T], max [T], sum exp(z - max) [T]} for a whole vocabulary; with `raw`, of the columns [col0, col0 + V) that this
+// rank holds of `vocab`, and the label's logit (0 where another rank holds it) in place of the loss.
+std::vector<at::Tensor> linear_ce_fwd(at::Tensor x, at::Tensor w, at::Tensor labels, int64_t col0, int64_t vocab,
+                                      int64_t ignore, bool raw) {
+  check_ce(x, w, labels);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t T = x.size(0), V = w.size(0);
+  TORCH_CHECK(V > 0 && col0 >= 0 && col0 + V <= vocab && (raw || V == vocab), "columns outside the vocabulary");
+  auto f32 = x.options().dtype(at::kFloat);
+  auto out = at::empty({3, T}, f32);
+  if (T == 0) return out.unbind(0);
+  const int64_t tiles = (V + 255) / 256;
+  auto part = at::empty({tiles, T, 2}, f32), target = at::empty({T}, f32);
+  CeArgs ce = ce_args(labels, col0, vocab, ignore);
+  ce.part = reinterpret_cast<float2*>(part.data_ptr<float>());
+  ce.target = target.data_ptr<float>();
+  linear_ce_gemm(tma_rows(x), tma_rows(w), ce, false, at::Tensor());
+  float* o = out.data_ptr<float>();
+  ce_join_kernel<<<(int)((T + 31) / 32), 1024, 0, cur_stream()>>>(ce, (int)T, (int)tiles, (int)V, raw, o, o + T,
+                                                                  o + 2 * T);
+  EMB_LAUNCH_CHECK();
+  count_launch();
+  return out.unbind(0);
+}
+
+// {dx [T, H] bf16, dw [V, H] bf16}, each undefined where it is not wanted; with `dw_accum` (fp32 [V, H]) the weight
+// gradient is added there.  `piece`: columns of a piece (0: as many as fit the workspace).
+std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor w, at::Tensor labels, at::Tensor top,
+                                      at::Tensor sum, int64_t col0, int64_t vocab, int64_t ignore, bool want_dx,
+                                      bool want_dw, c10::optional<at::Tensor> dw_accum, int64_t piece) {
+  check_ce(x, w, labels);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t T = x.size(0), V = w.size(0), H = x.size(1);
+  auto f32 = x.options().dtype(at::kFloat);
+  for (const auto& t : {top, sum})
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == T && t.device() == x.device(),
+                "the statistics of the forward pass must be fp32 [T]");
+  auto g = dloss.to(at::kFloat).contiguous();
+  TORCH_CHECK(g.numel() == T && g.device() == x.device(), "dloss must be [T]");
+  at::Tensor dx, dw;
+  if (dw_accum.has_value()) {
+    TORCH_CHECK(dw_accum->scalar_type() == at::kFloat && dw_accum->dim() == 2 && dw_accum->size(0) == V &&
+                    dw_accum->size(1) == H && dw_accum->stride(1) == 1 && dw_accum->device() == x.device(),
+                "the weight gradient accumulator must be fp32 [V, H]");
+  } else if (want_dw) {
+    dw = at::empty({V, H}, x.options());
+  }
+  if (want_dx) dx = at::empty({T, H}, x.options());
+  if (T == 0) {
+    if (dw.defined()) dw.zero_();
+    return {dx, dw};
+  }
+  auto xr = tma_rows(x), wr = tma_rows(w);
+  const int64_t whole = (V + 255) / 256 * 256;
+  if (piece <= 0) piece = kPieceBytes / (2 * T);
+  piece = std::min(whole, std::max<int64_t>(256, piece / 256 * 256));
+  const int64_t pieces = (V + piece - 1) / piece;
+  auto P = at::empty({T, piece}, x.options());
+  CeArgs ce = ce_args(labels, col0, vocab, ignore);
+  ce.top = top.data_ptr<float>();
+  ce.sum = sum.data_ptr<float>();
+  ce.dloss = g.data_ptr<float>();
+  // dx of few rows has few output tiles and a long sum: split the sum over the SMs (fp32 parts joined in order)
+  const int64_t tiles1 = ((T + 127) / 128) * ((H + 255) / 256);
+  const bool split = want_dx && tiles1 * 2 <= num_sms() && V > 512;
+  // shares of a piece of n columns: one output tile for every SM, at least 512 columns a share
+  auto shares = [&](int64_t n) { return std::max<int64_t>(1, std::min<int64_t>(num_sms() / tiles1, n / 512)); };
+  const int64_t n_parts = split ? (pieces - 1) * shares(piece) + shares(V - (pieces - 1) * piece) : 1;
+  at::Tensor parts;
+  if (want_dx && (split || pieces > 1)) parts = at::empty({n_parts, T, H}, f32);
+  int64_t part = 0;
+  for (int64_t i = 0; i < pieces; ++i) {
+    const int64_t v0 = i * piece, n = std::min(piece, V - v0);
+    auto Pi = P.narrow(1, 0, n), wi = wr.narrow(0, v0, n);
+    ce.col0 = col0 + v0;
+    linear_ce_gemm(xr, wi, ce, true, Pi);
+    if (want_dx) {
+      if (split) {
+        gemm_split_k(Pi, wi, parts.narrow(0, part, shares(n)));
+        part += shares(n);
+      } else {
+        gemm_tc(Pi, wi, false, false, pieces > 1 ? parts[0] : dx, i > 0, 0);
+      }
+    }
+    if (dw_accum.has_value()) gemm_tc(Pi, xr, true, false, dw_accum->narrow(0, v0, n), true, 0);
+    else if (want_dw) gemm_tc(Pi, xr, true, false, dw.narrow(0, v0, n), false, 0);
+  }
+  if (parts.defined()) {
+    const int64_t vecs = T * H / 4;
+    const int grid = (int)std::min<int64_t>((vecs + 255) / 256, (int64_t)num_sms() * 8);
+    parts_sum_kernel<<<grid, 256, 0, cur_stream()>>>(
+        reinterpret_cast<const float4*>(parts.data_ptr()), (int)n_parts, vecs,
+        reinterpret_cast<__nv_bfloat16*>(dx.data_ptr()));
+    EMB_LAUNCH_CHECK();
+    count_launch();
+  }
+  return {dx, dw};
+}
+
+}  // namespace emb

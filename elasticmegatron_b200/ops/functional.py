@@ -665,6 +665,90 @@ def vocab_parallel_cross_entropy(logits, labels, vocab_start, group):
     return VocabParallelCE.apply(logits, labels, vocab_start, group)
 
 
+# ------------------------------------------------------------------------------------------ linear cross entropy
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """Output layer and cross entropy without the logits (``csrc/gemm/linear_ce.cu``); see
+    :func:`linear_cross_entropy`.  The collectives are those of the output layer's linear (``mode``) and of the
+    vocab-parallel softmax statistics."""
+
+    @staticmethod
+    def forward(ctx, x, w, labels, vocab_start, vocab, mode, group, ignore_index):
+        xf = _all_gather_dim0(x, group) if mode == "col_sp" else x
+        fwd = ext().linear_ce_fwd if use_native(xf) else ref.linear_ce_fwd
+        if mode is None:
+            loss, m, total = fwd(xf, w, labels, vocab_start, vocab, ignore_index, False)
+        else:
+            target, top, total = fwd(xf, w, labels, vocab_start, vocab, ignore_index, True)
+            m = top.clone()
+            dist.all_reduce(m, op=dist.ReduceOp.MAX, group=group)
+            # the label's logit relative to the maximum comes from the one rank that holds its row
+            local = labels - vocab_start
+            counts = (labels >= 0) & (labels < vocab) & (labels != ignore_index)
+            own = counts & (local >= 0) & (local < w.shape[0])
+            st = torch.stack([total * torch.exp(top - m), torch.where(own, target - m, torch.zeros_like(m))])
+            dist.all_reduce(st, group=group)
+            total = st[0]
+            loss = torch.where(counts, torch.log(total) - st[1], torch.zeros_like(m))
+        ctx.save_for_backward(x, w, labels, m, total)
+        ctx.rest = (vocab_start, vocab, ignore_index)
+        ctx.mode, ctx.group = mode, group
+        return loss
+
+    @staticmethod
+    def backward(ctx, dloss):
+        x, w, labels, m, total = ctx.saved_tensors
+        mode, group = ctx.mode, ctx.group
+        want_dx, want_dw = ctx.needs_input_grad[:2]
+        xf = _all_gather_dim0(x, group) if mode == "col_sp" else x
+        mg = getattr(w, "main_grad", None) if want_dw else None
+        bwd = ext().linear_ce_bwd if use_native(xf) else ref.linear_ce_bwd
+        dx, dw = bwd(dloss, xf, w, labels, m, total, *ctx.rest, want_dx, want_dw,
+                     mg.view(w.shape) if mg is not None else None, LINEAR_CE_PIECE)
+        if want_dx and mode == "col_sp":
+            dx = _reduce_scatter_dim0(dx, group)
+        elif want_dx and mode == "col":
+            dx = _all_reduce(dx, group)
+        if mg is not None and getattr(w, "_grad_ready", None) is not None:
+            w._grad_ready()
+        return dx, dw, None, None, None, None, None, None
+
+
+# Columns of the vocabulary that the backward of linear_cross_entropy takes at a time (0: as many as fit 256 MiB).
+LINEAR_CE_PIECE = 0
+
+
+def linear_cross_entropy(x, w, labels, vocab_start: int = 0, mode: Optional[str] = None, group=None,
+                         ignore_index: int = -100):
+    """Per-token cross entropy [T] (fp32) of ``softmax(x @ w.T)`` at ``labels``, without keeping the logits [T, V].
+
+    ``x`` [T, H] and ``w`` [V, H] (bf16 on CUDA, H a multiple of 8), ``labels`` int64 [T] of global ids.  The forward
+    product keeps the softmax statistics alone; the backward computes the logits again, a piece of the vocabulary at a
+    time (``LINEAR_CE_PIECE`` columns), so the memory beside the gradients is one [T, piece] bf16 buffer.  It costs 8
+    T V H operations a step where :func:`linear` followed by :func:`vocab_parallel_cross_entropy` costs 6.
+
+    Labels equal to ``ignore_index``, and any outside the vocabulary, have loss and gradient 0.  The weight gradient
+    accumulates in fp32 into ``main_grad`` where the weight has one.  With a tensor-parallel ``group`` the weight is this
+    rank's rows ``[vocab_start, vocab_start + V)`` (equal shares) and ``mode`` is that of the output layer: ``"col"`` or,
+    with x split along the sequence, ``"col_sp"`` (labels are then those of the whole sequence)."""
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"x must be [T, H] and w [V, H], got {tuple(x.shape)} and {tuple(w.shape)}")
+    if x.dtype != w.dtype:
+        raise ValueError(f"x and w must have the same type, got {x.dtype} and {w.dtype}")
+    if x.shape[1] == 0 or x.shape[1] % 8 or w.shape[0] == 0:
+        raise ValueError(f"H must be a multiple of 8 and the vocabulary not empty, got w {tuple(w.shape)}")
+    size = dist.get_world_size(group) if group is not None else 1
+    if size == 1:
+        mode = None
+    elif mode not in ("col", "col_sp"):
+        raise ValueError(f"mode must be col or col_sp with a tensor-parallel group, got {mode!r}")
+    tokens = x.shape[0] * (size if mode == "col_sp" else 1)
+    if labels.dtype != torch.int64 or tuple(labels.shape) != (tokens,):
+        raise ValueError(f"labels must be int64 [{tokens}], got {tuple(labels.shape)} {labels.dtype}")
+    if size == 1 and vocab_start != 0:
+        raise ValueError("vocab_start needs the group that holds the rest of the vocabulary")
+    return LinearCrossEntropyFn.apply(x, w, labels.contiguous(), vocab_start, w.shape[0] * size, mode, group, ignore_index)
+
+
 # ------------------------------------------------------------------------------------------ embedding
 class VocabParallelEmbedding(torch.autograd.Function):
     @staticmethod

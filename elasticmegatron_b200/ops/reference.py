@@ -210,3 +210,45 @@ def moe_route_bwd(logits, experts, dweights, dscore, sigmoid, renorm, scaling):
         g = ds + q
         dl = s * (g - (s * g).sum(-1, keepdim=True))
     return dl.to(logits.dtype)
+
+
+# ------------------------------------------------------------------------------------------ linear cross entropy
+def _ce_rows(labels, col0, vocab, ignore, V):
+    """(rows whose label counts, those whose label is one of the columns [col0, col0 + V), its column there)."""
+    counts = (labels >= 0) & (labels < vocab) & (labels != ignore)
+    own = counts & (labels >= col0) & (labels < col0 + V)
+    return counts, own, torch.where(own, labels - col0, torch.zeros_like(labels))
+
+
+def linear_ce_fwd(x, w, labels, col0, vocab, ignore, raw):
+    """(loss, maximum, sum of exponentials) over this rank's columns; with ``raw`` the label's logit (0 where another
+    rank holds it) in place of the loss."""
+    z = x.float() @ w.float().t()
+    m = z.max(-1).values
+    s = torch.exp(z - m[:, None]).sum(-1)
+    counts, own, col = _ce_rows(labels, col0, vocab, ignore, w.shape[0])
+    t = torch.where(own, z.gather(1, col[:, None]).squeeze(1), torch.zeros_like(m))
+    return (t if raw else torch.where(counts, torch.log(s) + (m - t), torch.zeros_like(m))), m, s
+
+
+def linear_ce_bwd(dloss, x, w, labels, top, total, col0, vocab, ignore, want_dx, want_dw, dw_accum, piece):
+    """(dx, dw), the logits computed again for ``piece`` columns of the vocabulary at a time (0: all)."""
+    V = w.shape[0]
+    counts, own, col = _ce_rows(labels, col0, vocab, ignore, V)
+    g = torch.where(counts, dloss.float(), torch.zeros_like(top))
+    xf = x.float()
+    dx = torch.zeros_like(xf)
+    dw = [] if dw_accum is None else None
+    for v0 in range(0, V, piece or V):
+        wf = w[v0:v0 + (piece or V)].float()
+        p = torch.exp(xf @ wf.t() - top[:, None]) * (g / total)[:, None]
+        here = torch.nonzero(own & (col >= v0) & (col < v0 + wf.shape[0])).squeeze(1)
+        p[here, col[here] - v0] -= g[here]
+        p[~counts] = 0.0
+        if want_dx:
+            dx += p @ wf
+        if dw_accum is not None:
+            dw_accum[v0:v0 + wf.shape[0]] += p.t() @ xf
+        elif want_dw:
+            dw.append((p.t() @ xf).to(w.dtype))
+    return dx.to(x.dtype) if want_dx else None, torch.cat(dw) if dw else None
