@@ -27,6 +27,7 @@ std::vector<torch::Tensor> heads_bwd(torch::Tensor dy, c10::optional<torch::Tens
                                      torch::Tensor sinv, int64_t nq, int64_t nk, bool interleaved,
                                      c10::optional<torch::Tensor> wq, c10::optional<torch::Tensor> wk, double eps,
                                      c10::optional<torch::Tensor> dwq_accum, c10::optional<torch::Tensor> dwk_accum);
+int64_t heads_error_flag();
 torch::Tensor ce_local_max(torch::Tensor logits);
 torch::Tensor ce_local_stats(torch::Tensor logits, torch::Tensor labels, torch::Tensor lmax, int64_t vstart);
 torch::Tensor ce_bwd(torch::Tensor logits, torch::Tensor labels, torch::Tensor lmax, torch::Tensor sumexp,
@@ -122,6 +123,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rope_fwd", &rope_fwd);
   m.def("heads_fwd", &heads_fwd);
   m.def("heads_bwd", &heads_bwd);
+  m.def("heads_error_flag", &heads_error_flag);
   m.def("ce_local_max", &ce_local_max);
   m.def("ce_local_stats", &ce_local_stats);
   m.def("ce_bwd", &ce_bwd);

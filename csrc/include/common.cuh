@@ -28,7 +28,7 @@ inline void count_launch(long long n = 1) { launch_counter().fetch_add(n, std::m
 // Device-side error words of the kernels with bounded waits: one zero-initialised int per (device, slot),
 // allocated on first use on each device and kept until exit, so a timeout or abort code recorded on one
 // device is never dropped when another device becomes current.
-enum ErrSlot { kErrGemm = 0, kErrAttnFwd = 1, kErrAttnBwd = 2, kErrComm = 3, kErrSlots = 8 };
+enum ErrSlot { kErrGemm = 0, kErrAttnFwd = 1, kErrAttnBwd = 2, kErrComm = 3, kErrHeads = 4, kErrSlots = 8 };
 constexpr int kMaxDevices = 64;
 inline int* device_err_flag(int slot) {
   static std::mutex mu;

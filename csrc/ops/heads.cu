@@ -133,6 +133,7 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 
 constexpr int kHeadThreads = 256;
+constexpr long long kStreamHeads = 8192;
 
 // One launch does all heads; the blocks are split between the classes (query, key, passing) in proportion to
 // their work, so that a block meets one weight vector and a lane always the same channels of it.
@@ -288,17 +289,403 @@ __global__ void __launch_bounds__(kHeadThreads) heads_kernel(HeadParams p) {
   }
 }
 
+// ------------------------------------------------------------------------------------------ streamed kernel
+// The same operator for dense tensors.  Memory bound, so the data must not wait for registers: every warp streams
+// tiles of at most 2 KB of consecutive heads through a ring of its own in shared memory (cp.async.bulk, an mbarrier a
+// stage), turns them in place and sends them out with a bulk store.  Values pass without an instruction.  No warp waits
+// for another; the loads of the next stages are in flight while a tile is worked on.
+constexpr int kTileBytes = 2048;
+constexpr int kStreamWarps = 8;
+constexpr unsigned kWaitPolls = 1u << 24;  // seconds of polling before a wait gives up
+
+struct FastDiv {  // n / d for n < 2^30
+  unsigned mul, shift, d;
+  __device__ __forceinline__ unsigned div(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+FastDiv fast_div(unsigned d) {
+  unsigned s = 0;
+  while ((1ull << s) < d) ++s;
+  return {(unsigned)((((1ull << s) - d) << 32) / d + 1), s, d};
+}
+
+struct StreamParams {
+  const void* x;
+  const void* dy;
+  void* out;
+  const float* cosv;
+  const float* sinv;
+  const void* w[2];
+  float* part;  // [blocks, 2, d]
+  int* err;
+  FastDiv per_token, slots, rows;  // heads of a token, of a group; tokens that share a row of the tables
+  int d, r, nq, nk;
+  unsigned heads, tile_heads, tiles;
+  float eps, inv_d;
+};
+
+__device__ __forceinline__ unsigned smem_at(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_at(dst)),
+               "l"(src), "r"(bytes), "r"(smem_at(bar))
+               : "memory");
+}
+__device__ __forceinline__ bool bulk_wait(uint64_t* bar, unsigned parity) {
+  for (unsigned i = 0; i < kWaitPolls; ++i) {
+    unsigned ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok)
+                 : "r"(smem_at(bar)), "r"(parity)
+                 : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+
+// Two fp32 in one 64-bit register, for the packed arithmetic of sm_100 (one instruction for both).
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 f2_of(float a, float b) {
+  f2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 f2_to(f2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f2 f2_mul(f2 a, f2 b) {
+  f2 v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) {
+  f2 v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+
+// 8 channels as 4 pairs
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, f2* v) {
+  if constexpr (sizeof(T) == 4) {
+    const ulonglong2* q = reinterpret_cast<const ulonglong2*>(p);
+    const ulonglong2 u0 = q[0], u1 = q[1];
+    v[0] = u0.x;
+    v[1] = u0.y;
+    v[2] = u1.x;
+    v[3] = u1.y;
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        v[i] = f2_of(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[i] = f2_of(f.x, f.y);
+      }
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const f2* v) {
+  if constexpr (sizeof(T) == 4) {
+    ulonglong2* q = reinterpret_cast<ulonglong2*>(p);
+    q[0] = make_ulonglong2(v[0], v[1]);
+    q[1] = make_ulonglong2(v[2], v[3]);
+  } else {
+    uint4 u;
+    unsigned* w = &u.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = f2_to(v[i]);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+        w[i] = *reinterpret_cast<const unsigned*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(f.x, f.y);
+        w[i] = *reinterpret_cast<const unsigned*>(&h);
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = u;
+  }
+}
+
+// 4 cosines and sines from column `col` of a row of the tables
+__device__ __forceinline__ void load4(const StreamParams& p, unsigned row, int col, f2* c, f2* s) {
+  const size_t at = (size_t)row * (p.r / 2) + col;
+  const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(p.cosv + at), v = *reinterpret_cast<const ulonglong2*>(p.sinv + at);
+  c[0] = u.x;
+  c[1] = u.y;
+  s[0] = v.x;
+  s[1] = v.y;
+}
+
+// The two vectors of 8 channels that lane `pair` holds of its head, as channel offsets, and whether each turns.
+template <bool INTER>
+__device__ __forceinline__ void vectors_of(int pair, int d, int r, int& a, int& b, bool& ta, bool& tb) {
+  if constexpr (INTER) {  // pairs lie inside a vector; neighbouring lanes take neighbouring vectors (no bank conflicts)
+    a = pair * 8;
+    b = a + (d / 8 + 1) / 2 * 8;
+    ta = a < r;
+    tb = b < r;
+  } else {
+    const int hv = r / 16;
+    ta = tb = pair < hv;
+    a = ta ? pair * 8 : r + 2 * (pair - hv) * 8;
+    b = ta ? (pair + hv) * 8 : a + 8;
+  }
+}
+
+// A lane works on 16 channels of a head in packed fp32.  Every warp takes consecutive tiles, so a lane meets the heads
+// of one token one after the other and loads the token's cosines and sines once; the norm weights sit in shared memory
+// as fp32, [class][quarter][lane] so that a lane's four 16-byte reads are free of bank conflicts.  What keeps the
+// kernel from the memory's rate otherwise is the number of instructions: 4 heads of 128 channels have about 350 issue
+// slots forward and 500 backward at the rate of a plain copy.
+template <typename T, int LPH, int STAGES, bool INTER, bool NORM, bool BWD>
+__global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 3) heads_stream_kernel(StreamParams p) {
+  constexpr int HPW = 32 / LPH;
+  constexpr int BUFS = NORM && BWD ? 2 : 1;  // dy (or x), and x
+  extern __shared__ __align__(128) uint8_t s_ring[];
+  __shared__ uint64_t s_bar[kStreamWarps][STAGES];
+  __shared__ __align__(16) float s_w[NORM ? 2 : 1][4][LPH][4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % LPH, sub = lane / LPH;
+  uint8_t* ring = s_ring + warp * (STAGES * BUFS * kTileBytes);
+  uint64_t* bar = s_bar[warp];
+  const unsigned head_bytes = p.d * (unsigned)sizeof(T);
+  const unsigned long long warps = (unsigned long long)gridDim.x * kStreamWarps, me = blockIdx.x * kStreamWarps + warp;
+  const unsigned first = (unsigned)(p.tiles * me / warps), last = (unsigned)(p.tiles * (me + 1) / warps);
+  const char* src0 = reinterpret_cast<const char*>(BWD ? p.dy : p.x);
+  const char* src1 = reinterpret_cast<const char*>(p.x);
+
+  int oa, ob;
+  bool ta, tb;
+  vectors_of<INTER>(l, p.d, p.r, oa, ob, ta, tb);
+  const int pairs = (p.d / 8 + 1) / 2;  // lanes past them hold nothing
+  const bool ha = l < pairs && oa < p.d, hb = l < pairs && ob < p.d;
+  ta = ta && ha;
+  tb = tb && hb;
+  const bool full = pairs == LPH && p.d % 16 == 0;  // every lane holds two vectors
+  if (!ha) oa = 0;
+  if (!hb) ob = 0;
+
+  auto load = [&](unsigned tile, int st) {  // lane 0
+    const unsigned h0 = tile * p.tile_heads, n = min(p.tile_heads, p.heads - h0), bytes = n * head_bytes;
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(bar + st)), "r"(bytes * BUFS)
+                 : "memory");
+    bulk_load(ring + st * BUFS * kTileBytes, src0 + (size_t)h0 * head_bytes, bytes, bar + st);
+    if (BUFS == 2) bulk_load(ring + (st * BUFS + 1) * kTileBytes, src1 + (size_t)h0 * head_bytes, bytes, bar + st);
+  };
+
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_at(bar + i)));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i)
+      if (first + i < last) load(first + i, i);
+  }
+  f2 gw[NORM && BWD ? 2 : 1][8];
+  if constexpr (NORM) {
+    if (threadIdx.x < 2 * LPH) {  // thread (class, l) lays out that lane's weights
+      const int c = threadIdx.x / LPH, q = threadIdx.x % LPH;
+      int qa, qb;
+      bool qt;
+      vectors_of<INTER>(q, p.d, p.r, qa, qb, qt, qt);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int ch = (j < 8 ? qa : qb) + (j & 7);
+        s_w[c][j / 4][q][j & 3] = q < pairs && ch < p.d ? to_f<T>(reinterpret_cast<const T*>(p.w[c])[ch]) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < (BWD ? 2 : 1); ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gw[c][j] = 0ull;
+    __syncthreads();
+  } else {
+    __syncwarp();
+  }
+
+  unsigned have = ~0u;  // table row in cs / sn
+  f2 cs[4], sn[4];
+  unsigned it = 0;
+  for (unsigned tile = first; tile < last; ++tile, ++it) {
+    const int st = it % STAGES;
+    if (!bulk_wait(bar + st, (it / STAGES) & 1)) {
+      // a copy that does not arrive: report it, and leave after a bounded wait for the copies in flight
+      if (lane == 0) atomicExch(p.err, 1);
+      for (int i = 0; i < STAGES; ++i) bulk_wait(bar + i, ((it + i) / STAGES) & 1);
+      break;
+    }
+    uint8_t* buf = ring + st * BUFS * kTileBytes;
+    const unsigned h0 = tile * p.tile_heads, n = min(p.tile_heads, p.heads - h0);
+#pragma unroll 1
+    for (unsigned i0 = 0; i0 < n; i0 += HPW) {
+      // heads past the end and values are read like any other (whatever the stage holds) but neither counted nor written
+      const unsigned i = i0 + sub, h = h0 + i;
+      const unsigned slot = h - p.slots.div(h) * p.slots.d;
+      const bool live = i < n && slot < (unsigned)(p.nq + p.nk);
+      const bool is_k = slot >= (unsigned)p.nq;
+      T* va = reinterpret_cast<T*>(buf + i * head_bytes) + oa;
+      T* vb = reinterpret_cast<T*>(buf + i * head_bytes) + ob;
+      const unsigned row = p.rows.div(p.per_token.div(h));
+      if (live && row != have) {
+        have = row;
+        if constexpr (INTER) {
+          if (ta) load4(p, row, oa / 2, cs, sn);
+          if (tb) load4(p, row, ob / 2, cs + 2, sn + 2);
+        } else if (ta) {
+          load4(p, row, oa, cs, sn);
+          load4(p, row, oa + 4, cs + 2, sn + 2);
+        }
+      }
+      f2 a[8], x[8];
+      load8<T>(va, a);
+      load8<T>(vb, a + 4);
+      if constexpr (NORM && BWD) {
+        load8<T>(va + kTileBytes / sizeof(T), x);
+        load8<T>(vb + kTileBytes / sizeof(T), x + 4);
+      }
+      if (!full) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (!(j < 4 ? ha : hb)) {
+            a[j] = 0ull;
+            if (NORM && BWD) x[j] = 0ull;
+          }
+        }
+      }
+      auto turn = [&](f2* v) {
+        if constexpr (INTER) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (j < 4 ? ta : tb) {
+              const float2 c = f2_to(cs[j / 2]), s = f2_to(sn[j / 2]), u = f2_to(v[j]);
+              const float cj = j & 1 ? c.y : c.x, sj = j & 1 ? s.y : s.x;
+              v[j] = BWD ? f2_of(u.x * cj + u.y * sj, u.y * cj - u.x * sj) : f2_of(u.x * cj - u.y * sj, u.y * cj + u.x * sj);
+            }
+          }
+        } else if (ta) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f2 u = v[j], w = v[4 + j], neg = f2_mul(sn[j], f2_of(-1.f, -1.f));
+            v[j] = f2_fma(w, BWD ? sn[j] : neg, f2_mul(u, cs[j]));
+            v[4 + j] = f2_fma(u, BWD ? neg : sn[j], f2_mul(w, cs[j]));
+          }
+        }
+      };
+      if constexpr (NORM) {
+        const f2* y = BWD ? x : a;
+        f2 ss = 0ull;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = f2_fma(y[j], y[j], ss);
+        const float2 s2 = f2_to(ss);
+        const float rstd = rsqrtf(group_sum<LPH>(s2.x + s2.y) * p.inv_d + p.eps);
+        const f2 r2 = f2_of(rstd, rstd);
+        const float* wl = &s_w[is_k ? 1 : 0][0][l][0];
+        f2 w[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(wl + q * LPH * 4);
+          w[2 * q] = u.x;
+          w[2 * q + 1] = u.y;
+        }
+        if constexpr (!BWD) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a[j] = f2_mul(f2_mul(a[j], r2), w[j]);
+          turn(a);
+        } else {
+          turn(a);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = f2_mul(x[j], r2);
+          if (live) {
+            if (is_k) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) gw[1][j] = f2_fma(a[j], x[j], gw[1][j]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) gw[0][j] = f2_fma(a[j], x[j], gw[0][j]);
+            }
+          }
+          f2 dot = 0ull;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            a[j] = f2_mul(a[j], w[j]);
+            dot = f2_fma(a[j], x[j], dot);
+          }
+          const float2 d2 = f2_to(dot);
+          const float m = group_sum<LPH>(d2.x + d2.y) * -p.inv_d;
+          const f2 m2 = f2_of(m, m);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a[j] = f2_mul(f2_fma(x[j], m2, a[j]), r2);
+        }
+      } else {
+        turn(a);
+      }
+      if (live && ha) store8<T>(va, a);
+      if (live && hb) store8<T>(vb, a + 4);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                       reinterpret_cast<char*>(p.out) + (size_t)h0 * head_bytes),
+                   "r"(smem_at(buf)), "r"(n * head_bytes)
+                   : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      // the stage of the tile before this one is free once its store has read it
+      if (it > 0 && tile + STAGES - 1 < last) {
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        load(tile + STAGES - 1, (it - 1) % STAGES);
+      }
+    }
+    __syncwarp();
+  }
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  if constexpr (NORM && BWD) {
+    __syncthreads();  // every ring is done with: [warps, 2, d] sums of the weight gradients take its place
+    float* s_dw = reinterpret_cast<float*>(s_ring);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float2 v = f2_to(gw[c][j]);
+#pragma unroll
+        for (int o = LPH; o < 32; o <<= 1) {
+          v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+          v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+        }
+        const int ch = (j < 4 ? oa : ob) + 2 * (j & 3);
+        if (sub == 0 && (j < 4 ? ha : hb)) *reinterpret_cast<float2*>(&s_dw[(warp * 2 + c) * p.d + ch]) = v;
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * p.d; i += kStreamWarps * 32) {
+      float v = 0.f;
+#pragma unroll
+      for (int q = 0; q < kStreamWarps; ++q) v += s_dw[q * 2 * p.d + i];
+      p.part[(size_t)blockIdx.x * 2 * p.d + i] = v;
+    }
+  }
+}
+
 // dw[cls][c] (+)= sum over the class's blocks of part[block][c]: 32 channels a CTA, 32 slices of the blocks, each
 // slice summed in order and the slices joined by a fixed tree.
 template <typename T>
-__global__ void __launch_bounds__(1024) heads_join_kernel(const float* __restrict__ part, int d, int nb0, int nb1,
+__global__ void __launch_bounds__(1024) heads_join_kernel(const float* __restrict__ part, int d, int nb0, int nb1, int both,
                                                           T* dw0, T* dw1, float* acc0, float* acc1) {
   __shared__ float sh[32][33];
-  const int cls = blockIdx.y, b0 = cls ? nb0 : 0, b1 = cls ? nb0 + nb1 : nb0;
+  // rows of `part`: those of class 0 and then those of class 1, or (`both`) the two of each block side by side
+  const int cls = blockIdx.y, by = both ? 2 : 1;
+  const int b0 = both ? 0 : cls ? nb0 : 0, b1 = both ? nb0 : cls ? nb0 + nb1 : nb0, shift = both ? cls : 0;
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float v = 0.f;
   if (c < d)
-    for (int b = b0 + slice; b < b1; b += 32) v += part[(long long)b * d + c];
+    for (int b = b0 + slice; b < b1; b += 32) v += part[((long long)b * by + shift) * d + c];
   sh[slice][lane] = v;
   __syncthreads();
   v = warp_sum(sh[lane][slice]);  // slices of channel blockIdx.x * 32 + slice
@@ -422,6 +809,78 @@ int split_grid(HeadParams& p, bool vec, int waves) {
   return at;
 }
 
+template <typename T, int LPH, bool INTER, bool NORM, bool BWD>
+void launch_stream(const StreamParams& p, int grid) {
+  constexpr int kStages = NORM && BWD ? 3 : 4;
+  constexpr int kSmem = kStreamWarps * kStages * kTileBytes * (NORM && BWD ? 2 : 1);
+  auto kern = heads_stream_kernel<T, LPH, kStages, INTER, NORM, BWD>;
+  static bool done[kMaxDevices] = {};  // the shared-memory limit belongs to the device's context
+  int dev = 0;
+  EMB_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!done[dev]) {
+    EMB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    done[dev] = true;
+  }
+  kern<<<grid, kStreamWarps * 32, kSmem, cur_stream()>>>(p);
+}
+
+template <typename T, int LPH>
+void pick_stream_mode(const StreamParams& p, int grid, bool inter, bool norm, bool bwd) {
+  if (inter) {
+    if (norm) bwd ? launch_stream<T, LPH, true, true, true>(p, grid) : launch_stream<T, LPH, true, true, false>(p, grid);
+    else bwd ? launch_stream<T, LPH, true, false, true>(p, grid) : launch_stream<T, LPH, true, false, false>(p, grid);
+  } else {
+    if (norm) bwd ? launch_stream<T, LPH, false, true, true>(p, grid) : launch_stream<T, LPH, false, true, false>(p, grid);
+    else bwd ? launch_stream<T, LPH, false, false, true>(p, grid) : launch_stream<T, LPH, false, false, false>(p, grid);
+  }
+}
+
+template <typename T>
+void pick_stream(const StreamParams& p, int grid, bool inter, bool norm, bool bwd) {
+  switch (lanes_per_head(p.d, 8)) {
+    case 1: case 2: case 4: return pick_stream_mode<T, 4>(p, grid, inter, norm, bwd);
+    case 8: return pick_stream_mode<T, 8>(p, grid, inter, norm, bwd);
+    case 16: return pick_stream_mode<T, 16>(p, grid, inter, norm, bwd);
+    default: return pick_stream_mode<T, 32>(p, grid, inter, norm, bwd);
+  }
+}
+
+// Dense tensors with 16-byte rows are streamed once there is more than a tile for every warp of the direct kernel.
+bool streams(const HeadParams& p, bool vec, const at::Tensor& t, const at::Tensor& other) {
+  return vec && t.is_contiguous() && (!other.defined() || other.is_contiguous()) &&
+         p.tokens * p.G * p.S >= kStreamHeads;
+}
+
+StreamParams stream_params(const HeadParams& p, int esize) {
+  StreamParams q{};
+  q.x = p.x;
+  q.dy = p.dy;
+  q.out = p.out;
+  q.cosv = p.cosv;
+  q.sinv = p.sinv;
+  q.w[0] = p.w[0];
+  q.w[1] = p.w[1];
+  q.err = device_err_flag(kErrHeads);
+  q.per_token = fast_div((unsigned)(p.G * p.S));
+  q.slots = fast_div((unsigned)p.S);
+  q.rows = fast_div(p.tb ? 1u : (unsigned)p.B);
+  q.d = p.d;
+  q.r = p.r;
+  q.nq = p.n[0];
+  q.nk = p.n[1];
+  q.eps = p.eps;
+  q.inv_d = 1.f / (float)p.d;
+  q.heads = (unsigned)(p.tokens * p.G * p.S);
+  const unsigned hpw = 32u / std::max(4, lanes_per_head(p.d, 8));
+  q.tile_heads = std::max(hpw, kTileBytes / (unsigned)(p.d * esize) / hpw * hpw);
+  q.tiles = (q.heads + q.tile_heads - 1) / q.tile_heads;
+  return q;
+}
+
+int stream_grid(const StreamParams& q, int ctas_per_sm) {
+  return (int)std::min<long long>((q.tiles + kStreamWarps - 1) / kStreamWarps, (long long)num_sms() * ctas_per_sm);
+}
+
 template <typename F>
 void by_type(at::ScalarType t, F f) {
   if (t == at::kBFloat16) f(__nv_bfloat16{});
@@ -463,6 +922,13 @@ at::Tensor heads_fwd(at::Tensor qkv, at::Tensor cosv, at::Tensor sinv, int64_t n
   p.out = out.data_ptr();
   p.eps = (float)eps;
   vec = vec && rows_aligned(x);
+  if (streams(p, vec, x, at::Tensor())) {
+    const StreamParams q = stream_params(p, (int)x.element_size());
+    by_type(x.scalar_type(), [&](auto t) { pick_stream<decltype(t)>(q, stream_grid(q, 3), interleaved, norm, false); });
+    EMB_LAUNCH_CHECK();
+    count_launch();
+    return out;
+  }
   const int grid = split_grid(p, vec, kHeadWaves);
   by_type(x.scalar_type(), [&](auto t) { pick_shape<decltype(t)>(p, grid, vec, interleaved, norm, false); });
   EMB_LAUNCH_CHECK();
@@ -526,24 +992,34 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
   p.out = dx.data_ptr();
   p.eps = (float)eps;
   vec = vec && rows_aligned(g);
-  const int grid = split_grid(p, vec, kHeadWaves);
+  const bool stream = streams(p, vec, g, x);
+  StreamParams q{};
+  if (stream) q = stream_params(p, (int)g.element_size());
+  const int grid = stream ? stream_grid(q, norm ? 2 : 3) : split_grid(p, vec, kHeadWaves);
+  const int nb0 = stream ? grid : p.block0[1], nb1 = stream ? grid : p.block0[2] - p.block0[1];
   at::Tensor part;
-  const int nb0 = p.block0[1], nb1 = p.block0[2] - p.block0[1];
   if (norm) {
     part = at::empty({nb0 + nb1, p.d}, g.options().dtype(at::kFloat));
-    p.part = part.data_ptr<float>();
+    p.part = q.part = part.data_ptr<float>();
   }
   by_type(g.scalar_type(), [&](auto t) {
     using T = decltype(t);
-    pick_shape<T>(p, grid, vec, interleaved, norm, true);
+    if (stream) pick_stream<T>(q, grid, interleaved, norm, true);
+    else pick_shape<T>(p, grid, vec, interleaved, norm, true);
     if (norm) {
       heads_join_kernel<T><<<dim3((p.d + 31) / 32, 2), 1024, 0, cur_stream()>>>(
-          p.part, p.d, nb0, nb1, (T*)dw[0], (T*)dw[1], acc[0], acc[1]);
+          p.part, p.d, nb0, nb1, stream, (T*)dw[0], (T*)dw[1], acc[0], acc[1]);
     }
   });
   EMB_LAUNCH_CHECK();
   count_launch(norm ? 2 : 1);
   return res;
+}
+
+int64_t heads_error_flag() {
+  int v = 0;
+  EMB_CUDA_CHECK(cudaMemcpy(&v, device_err_flag(kErrHeads), sizeof(int), cudaMemcpyDeviceToHost));
+  return v;
 }
 
 }  // namespace emb
