@@ -22,9 +22,11 @@
 //   softmax: dl_e = s_e (ds_e + q_e - sum_f s_f (ds_f + q_f))
 //   sigmoid: dl_e = s_e (1 - s_e) (ds_e + (q_e - sum_f q_f p_f) / (sum s + 1e-20))
 //
-// One warp per token, lane i holding experts [i EPL, (i + 1) EPL): the logits are read once, everything else stays in
-// registers, and a round of the selection is one redux over order-preserving integer keys.  The statistics are
-// kept per lane over the warp's tokens, joined over the warps of a CTA and then over the CTAs in a fixed order.
+// One warp per token, lane i holding experts [i EPL, (i + 1) EPL): the logits are read once and the scores stay in
+// registers.  The kernels have few bytes and many instructions for a token, so these are what is kept low: each lane
+// sorts its keys (integers in the order of the choice) once, a round of the selection is then one redux over the lanes'
+// first keys, and the chosen indices and scores are looked up afterwards by k lanes at once through shared memory.  The
+// statistics are kept per lane over the warp's tokens and joined over the warps and the CTAs in a fixed order.
 #include "../include/common.cuh"
 
 #include <c10/cuda/CUDAGuard.h>
@@ -43,6 +45,8 @@ struct RouteParams {
   long long ld;  // elements between rows
   const float* bias;
   int T, E, k, groups, topg, gbest;
+  int glanes;   // lanes that value a group
+  int gstride;  // words between groups in shared memory: the lanes of all groups hit different banks
   float scaling;
   int sigmoid, renorm;
   // forward
@@ -56,9 +60,6 @@ struct RouteParams {
   const int* chosen;
   void* dlogits;
 };
-
-template <typename T>
-__device__ __forceinline__ float load_f(const T* p) { return (float)*p; }
 
 __device__ __forceinline__ float quot(float a, float b) { return __fdiv_rn(a, b); }
 
@@ -75,19 +76,37 @@ __device__ __forceinline__ unsigned order_key(float c) {
   return c > -INFINITY ? o : 1u;
 }
 
-// The lane's scores s[j] of its EPL experts.  Returns what the sigmoid divides its normalised scores by.
-template <int EPL>
-__device__ __forceinline__ float scores(const float* l, float* s, int sigmoid) {
-  if (sigmoid) {
-    float t = 0.f;
+template <typename T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
+  T v[N];
+};
+
+// The lane's EPL logits of a row, -inf past the last expert.  VEC: experts fill whole lanes and rows are aligned, so a
+// lane reads and writes its share in one piece.
+template <typename T, int EPL, bool VEC>
+__device__ __forceinline__ void load_row(const T* row, int E, int lane, float* l) {
+  if constexpr (VEC) {
+    if (lane * EPL < E) {
+      const Pack<T, EPL> v = reinterpret_cast<const Pack<T, EPL>*>(row)[lane];
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) l[j] = (float)v.v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) l[j] = -INFINITY;
+    }
+  } else {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      s[j] = quot(1.f, 1.f + expf(-l[j]));
-      t += s[j];
+      const int e = lane * EPL + j;
+      l[j] = e < E ? (float)row[e] : -INFINITY;
     }
-    return warp_sum(t) + kTiny;
   }
-  float mx = l[0];
+}
+
+// Maximum of the row and the 64-bit sum of its exponentials, rounded to fp32 (1 for an all-masked row); s = exponentials.
+template <int EPL>
+__device__ __forceinline__ void softmax_parts(const float* l, float* s, float& mx, float& z) {
+  mx = l[0];
 #pragma unroll
   for (int j = 1; j < EPL; ++j) mx = fmaxf(mx, l[j]);
   mx = warp_max(mx);
@@ -97,138 +116,206 @@ __device__ __forceinline__ float scores(const float* l, float* s, int sigmoid) {
     s[j] = l[j] == -INFINITY ? 0.f : expf(l[j] - mx);
     sum += (double)s[j];
   }
-  const float z = (float)warp_sum_d(sum);
-  const float d = z == 0.f ? 1.f : z;  // an all-masked row
-#pragma unroll
-  for (int j = 0; j < EPL; ++j) s[j] = quot(s[j], d);
-  return 1.f;
+  z = (float)warp_sum_d(sum);
+  if (z == 0.f) z = 1.f;
 }
 
-template <typename T, int EPL>
-__device__ __forceinline__ void load_row(const RouteParams& p, int t, int lane, float* l) {
-  const T* row = reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld;
+// Falling order by a merge-exchange network (compile-time indices, so the keys stay in registers).
+template <int N>
+__device__ __forceinline__ void sort_keys(unsigned* k) {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int e = lane * EPL + j;
-    l[j] = e < p.E ? load_f(row + e) : -INFINITY;
+  for (int p = 1; p < N; p *= 2) {
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2) {
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q) {
+#pragma unroll
+        for (int i = 0; i < q; ++i) {
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const unsigned a = k[i + j], b = k[i + j + q];
+            k[i + j] = max(a, b);
+            k[i + j + q] = min(a, b);
+          }
+        }
+      }
+    }
   }
 }
 
-template <typename T, int EPL>
+template <typename T, int EPL, bool VEC>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_fwd_kernel(RouteParams p) {
-  extern __shared__ float s_mem[];  // [warps, E] score sums; [E] counts; [warps, E] choice values (groups)
+  // [warps, 32 EPL] keys, [warps, 32 EPL] scores (after the last token: score sums), [E] counts, [warps, groups, gstride]
+  extern __shared__ __align__(16) unsigned s_mem[];
+  constexpr int ROW = 32 * EPL;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int* s_cnt = reinterpret_cast<int*>(s_mem + kRouteWarps * p.E);
-  float* s_c = reinterpret_cast<float*>(s_cnt + p.E) + warp * p.E;
+  unsigned* s_key = s_mem + warp * ROW;
+  float* s_val = reinterpret_cast<float*>(s_mem + kRouteWarps * ROW) + warp * ROW;
+  int* s_cnt = reinterpret_cast<int*>(s_mem + 2 * kRouteWarps * ROW);
+  float* s_grp = reinterpret_cast<float*>(s_cnt + p.E) + warp * p.groups * p.gstride;
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) s_cnt[e] = 0;
   __syncthreads();
+  const bool by_group = p.groups > p.topg, by_logit = !p.bias && !by_group;
+  const int per = p.E / p.groups;
   float bias[EPL], acc[EPL];
+  int loc[EPL];  // expert's place in s_grp, and its group in the upper half
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     const int e = lane * EPL + j;
     bias[j] = p.bias && e < p.E ? p.bias[e] : 0.f;
     acc[j] = 0.f;
+    const int g = e < p.E ? e / per : 0;
+    loc[j] = (g * p.gstride + e - g * per) | (g << 16);
   }
-  const bool by_group = p.groups > p.topg, by_logit = !p.bias && !by_group;
   for (int t = blockIdx.x * kRouteWarps + warp; t < p.T; t += gridDim.x * kRouteWarps) {
-    float l[EPL], s[EPL];
+    float s[EPL];
     unsigned key[EPL];
-    load_row<T, EPL>(p, t, lane, l);
-    const float norm = scores<EPL>(l, s, p.sigmoid);
+    {
+      float l[EPL];
+      load_row<T, EPL, VEC>(reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld, p.E, lane, l);
+      if (p.sigmoid) {
+        float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const int e = lane * EPL + j;
-      if (e < p.E) acc[j] += p.sigmoid ? quot(s[j], norm) : s[j];
-      const float c = by_logit ? l[j] : l[j] > -INFINITY ? s[j] + bias[j] : -INFINITY;
-      key[j] = e < p.E ? order_key(c) : 0u;
-      if (by_group && e < p.E) s_c[e] = c;
-    }
-    if (by_group) {
-      __syncwarp();
-      // lane g values group g: its gbest largest, one after the other in falling order
-      unsigned gkey = 0u;
-      const int per = p.E / p.groups;
-      if (lane < p.groups) {
-        const float* c = s_c + lane * per;
-        float sum = 0.f, last = INFINITY;
-        int seen = 0, used = 0;  // values equal to `last` already taken
-        for (int m = 0; m < p.gbest; ++m) {
-          float best = -INFINITY;
-          int ties = 0;
-          for (int i = 0; i < per; ++i) {
-            const float v = c[i];
-            if (v == last) ++ties;
-            if (v < last && v > best) best = v;
-          }
-          if (used < ties) best = last;  // another copy of the value taken before
-          used = best == last ? used + 1 : 1;
-          last = best;
-          if (!(best > -INFINITY)) break;
-          sum = seen ? sum + best : best;
-          ++seen;
+        for (int j = 0; j < EPL; ++j) {
+          s[j] = __frcp_rn(1.f + expf(-l[j]));
+          sum += s[j];
         }
-        gkey = seen ? order_key(sum) : 1u;
-      }
-      unsigned kept = 0u;
-      for (int m = 0; m < p.topg; ++m) {
-        const unsigned top = __reduce_max_sync(kFull, gkey);
-        const int g = __ffs(__ballot_sync(kFull, gkey == top)) - 1;
-        kept |= 1u << g;
-        if (lane == g) gkey = 0u;
+        const float inv = __fdividef(1.f, warp_sum(sum) + kTiny);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) acc[j] += s[j] * inv;
+      } else {
+        float mx, z;
+        softmax_parts<EPL>(l, s, mx, z);
+        const float inv = quot(1.f, z);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+          s[j] = by_logit ? s[j] * inv : quot(s[j], z);
+          acc[j] += s[j];
+        }
       }
 #pragma unroll
       for (int j = 0; j < EPL; ++j) {
         const int e = lane * EPL + j;
-        if (e < p.E && !((kept >> (e / per)) & 1u)) key[j] = 0u;
+        const float c = by_logit ? l[j] : l[j] > -INFINITY ? s[j] + bias[j] : -INFINITY;
+        key[j] = e < p.E ? order_key(c) : 0u;
+        if (by_group && e < p.E) s_grp[loc[j] & 0xffff] = c;
       }
-      __syncwarp();
     }
-    float w = 0.f;
-    int mine = 0;
-    for (int r = 0; r < p.k; ++r) {
-      unsigned best = key[0];
-#pragma unroll
-      for (int j = 1; j < EPL; ++j) best = max(best, key[j]);
-      const unsigned top = __reduce_max_sync(kFull, best);
-      const int src = __ffs(__ballot_sync(kFull, best == top)) - 1;
-      float sv = 0.f;
-      int at = 0;
-      if (lane == src) {
-        bool open = true;
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) {
-          if (open && key[j] == top) {
-            sv = s[j];
-            at = j;
-            key[j] = 0u;
-            open = false;
+    if (by_group) {
+      __syncwarp();
+      // p.glanes lanes value a group, each from every glanes-th of its experts
+      const int g = lane / p.glanes, part = lane % p.glanes;
+      unsigned gkey = 0u;
+      float sum = 0.f;
+      bool any = false;
+      const float* c = s_grp + (g < p.groups ? g : 0) * p.gstride;
+      if (p.gbest <= 2) {
+        float b1 = -INFINITY, b2 = -INFINITY;  // the two largest (NaN is passed over)
+        for (int i = part; i < per; i += p.glanes) {
+          const float v = c[i];
+          b2 = fmaxf(b2, fminf(b1, v == v ? v : -INFINITY));
+          b1 = fmaxf(b1, v);
+        }
+        for (int o = 1; o < p.glanes; o <<= 1) {
+          const float o1 = __shfl_xor_sync(kFull, b1, o), o2 = __shfl_xor_sync(kFull, b2, o);
+          b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+          b1 = fmaxf(b1, o1);
+        }
+        any = b1 > -INFINITY;
+        sum = p.gbest == 2 && b2 > -INFINITY ? b1 + b2 : b1;
+      } else {
+        // one after the other in falling order; equal values are told apart by their place
+        float last = INFINITY;
+        int last_i = -1;
+        for (int m = 0; m < p.gbest; ++m) {
+          float best = -INFINITY;
+          int best_i = 0x7fffffff;
+          for (int i = part; i < per; i += p.glanes) {
+            const float v = c[i];
+            const bool open = v < last || (v == last && i > last_i);
+            if (open && v > best) {
+              best = v;
+              best_i = i;
+            }
           }
+          for (int o = 1; o < p.glanes; o <<= 1) {
+            const float ov = __shfl_xor_sync(kFull, best, o);
+            const int oi = __shfl_xor_sync(kFull, best_i, o);
+            if (ov > best || (ov == best && oi < best_i)) {
+              best = ov;
+              best_i = oi;
+            }
+          }
+          if (best > -INFINITY) {
+            sum = any ? sum + best : best;
+            any = true;
+          }
+          last = best;
+          last_i = best_i;
         }
       }
-      sv = __shfl_sync(kFull, sv, src);
-      at = src * EPL + __shfl_sync(kFull, at, src);
+      if (g < p.groups && part == 0) gkey = any ? order_key(sum) : 1u;
+      unsigned kept = 0u;
+      for (int m = 0; m < p.topg; ++m) {
+        const unsigned top = __reduce_max_sync(kFull, gkey);
+        const int at = __ffs(__ballot_sync(kFull, gkey == top)) - 1;
+        kept |= 1u << (at / p.glanes);
+        if (lane == at) gkey = 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < EPL; ++j)
+        if (!((kept >> (loc[j] >> 16)) & 1u)) key[j] = 0u;
+    }
+    // keys and scores for the look-up of the chosen, then the lane's keys in falling order: a round takes the largest
+    // of the lanes' first keys, and the lane that holds it moves up
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      s_key[lane * EPL + j] = key[j];
+      s_val[lane * EPL + j] = s[j];
+    }
+    sort_keys<EPL>(key);
+    unsigned my_key = 0u;
+    int my_src = 0;
+    for (int r = 0; r < p.k; ++r) {
+      const unsigned top = __reduce_max_sync(kFull, key[0]);
+      const int src = __ffs(__ballot_sync(kFull, key[0] == top)) - 1;
       if (lane == r) {
-        w = sv;
-        mine = at;
+        my_key = top;
+        my_src = src;
+      }
+      if (lane == src) {
+#pragma unroll
+        for (int j = 0; j + 1 < EPL; ++j) key[j] = key[j + 1];
+        key[EPL - 1] = 0u;
       }
     }
+    __syncwarp();
+    // lane r finds its expert: in lane my_src's share, the copy of my_key after those that earlier rounds took
+    const unsigned same = __match_any_sync(kFull, my_key) & __match_any_sync(kFull, my_src) & ((1u << lane) - 1u);
+    int skip = __popc(same), mine = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      if (s_key[my_src * EPL + j] == my_key) {
+        if (skip == 0) mine = my_src * EPL + j;
+        --skip;
+      }
+    }
+    float w = lane < p.k ? s_val[mine] : 0.f;
     if (p.renorm) w = quot(w, warp_sum(w) + kTiny);
     if (lane < p.k) {
       p.weights[(long long)t * p.k + lane] = w * p.scaling;
       p.experts[(long long)t * p.k + lane] = mine;
       atomicAdd(&s_cnt[mine], 1);  // whole numbers: any order gives the same counts
     }
+    __syncwarp();
   }
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int e = lane * EPL + j;
-    if (e < p.E) s_mem[warp * p.E + e] = acc[j];
-  }
+  for (int j = 0; j < EPL; ++j) s_val[lane * EPL + j] = acc[j];
   __syncthreads();
+  const float* sums = reinterpret_cast<const float*>(s_mem + kRouteWarps * ROW);
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
     float v = 0.f;
 #pragma unroll
-    for (int q = 0; q < kRouteWarps; ++q) v += s_mem[q * p.E + e];
+    for (int q = 0; q < kRouteWarps; ++q) v += sums[q * ROW + e];
     p.part[(long long)blockIdx.x * p.E + e] = v;
     p.cpart[(long long)blockIdx.x * p.E + e] = s_cnt[e];
   }
@@ -261,76 +348,84 @@ __global__ void __launch_bounds__(1024) route_join_kernel(const float* __restric
   }
 }
 
-template <typename T, int EPL>
+template <typename T, int EPL, bool VEC>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_bwd_kernel(RouteParams p) {
+  __shared__ __align__(16) float s_ds[kRouteWarps][32 * EPL];  // ds of the chosen experts, 0 elsewhere
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* row = s_ds[warp];
   float q[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     const int e = lane * EPL + j;
     q[j] = p.dscore && e < p.E ? p.dscore[e] : 0.f;
+    row[e] = 0.f;
   }
+  __syncwarp();
   for (int t = blockIdx.x * kRouteWarps + warp; t < p.T; t += gridDim.x * kRouteWarps) {
-    float l[EPL], s[EPL], ds[EPL];
-    load_row<T, EPL>(p, t, lane, l);
-    float a = 0.f;
-    int e_r = -1;
+    const T* logits = reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld;
+    float l[EPL], s[EPL];
+    load_row<T, EPL, VEC>(logits, p.E, lane, l);
+    // lane r has the r-th chosen expert: its gradient and its score
+    float a = 0.f, sr = 0.f, lr = -INFINITY;
+    int er = 0;
     if (lane < p.k) {
-      a = p.dweights ? p.dweights[(long long)t * p.k + lane] * p.scaling : 0.f;
-      e_r = p.chosen[(long long)t * p.k + lane];
+      er = p.chosen[(long long)t * p.k + lane];
+      lr = (float)logits[er];
+      if (p.dweights) a = p.dweights[(long long)t * p.k + lane] * p.scaling;
     }
-    const float norm = scores<EPL>(l, s, p.sigmoid);
+    float norm = 1.f, dsum = 0.f;  // dsum: s (1 - s) for the sigmoid is kept in l
+    if (p.sigmoid) {
+      float total = 0.f;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) ds[j] = 0.f;
-    float den = 1.f, dot = 0.f;
-    if (p.renorm) {
-      float sel = 0.f, prod = 0.f;  // sums over this lane's chosen experts
-      for (int r = 0; r < p.k; ++r) {
-        const int at = __shfl_sync(kFull, e_r, r) - lane * EPL;
-        const float ar = __shfl_sync(kFull, a, r);
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) {
-          if (at == j) {
-            sel += s[j];
-            prod += ar * s[j];
-          }
-        }
+      for (int j = 0; j < EPL; ++j) {
+        const float x = expf(-fabsf(l[j])), y = __frcp_rn(1.f + x);
+        s[j] = l[j] >= 0.f ? y : x * y;
+        l[j] = x * y * y;  // s (1 - s), without the difference
+        total += s[j];
+        dsum += q[j] * s[j];
       }
-      den = warp_sum(sel) + kTiny;
-      dot = quot(warp_sum(prod), den);
+      norm = quot(1.f, warp_sum(total) + kTiny);
+      dsum = warp_sum(dsum) * norm;
+      sr = __frcp_rn(1.f + expf(-lr));
+    } else {
+      float mx, z;
+      softmax_parts<EPL>(l, s, mx, z);
+      const float inv = quot(1.f, z);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        s[j] *= inv;
+        dsum += q[j] * s[j];
+      }
+      sr = lr == -INFINITY ? 0.f : expf(lr - mx) * inv;
     }
-    for (int r = 0; r < p.k; ++r) {
-      const int at = __shfl_sync(kFull, e_r, r) - lane * EPL;
-      const float ar = __shfl_sync(kFull, a, r);
+    float ds = a;
+    if (p.renorm) {
+      const float den = quot(1.f, warp_sum(lane < p.k ? sr : 0.f) + kTiny);
+      ds = (a - warp_sum(a * sr) * den) * den;
+    }
+    if (lane < p.k) {
+      row[er] = ds;
+      if (!p.sigmoid) dsum += sr * ds;
+    }
+    if (!p.sigmoid) dsum = warp_sum(dsum);
+    __syncwarp();
+    Pack<T, EPL> out;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      const float d = row[lane * EPL + j];
+      out.v[j] = (T)(p.sigmoid ? l[j] * (d + (q[j] - dsum) * norm) : s[j] * (d + q[j] - dsum));
+    }
+    __syncwarp();
+    if (lane < p.k) row[er] = 0.f;
+    T* dst = reinterpret_cast<T*>(p.dlogits) + (long long)t * p.E;
+    if constexpr (VEC) {
+      if (lane * EPL < p.E) reinterpret_cast<Pack<T, EPL>*>(dst)[lane] = out;
+    } else {
 #pragma unroll
       for (int j = 0; j < EPL; ++j)
-        if (at == j) ds[j] = quot(ar - dot, den);
+        if (lane * EPL + j < p.E) dst[lane * EPL + j] = out.v[j];
     }
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      if (p.sigmoid) {
-        sum += q[j] * s[j];
-      } else {
-        ds[j] += q[j];
-        sum += s[j] * ds[j];
-      }
-    }
-    sum = warp_sum(sum);
-    if (p.sigmoid) sum = quot(sum, norm);
-    T* out = reinterpret_cast<T*>(p.dlogits) + (long long)t * p.E;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const int e = lane * EPL + j;
-      float d;
-      if (p.sigmoid) {
-        const float x = expf(-fabsf(l[j]));  // s (1 - s) = x / (1 + x)^2, without the difference
-        d = quot(x, (1.f + x) * (1.f + x)) * (ds[j] + quot(q[j] - sum, norm));
-      } else {
-        d = s[j] * (ds[j] - sum);
-      }
-      if (e < p.E) out[e] = (T)d;
-    }
+    __syncwarp();
   }
 }
 
@@ -360,25 +455,41 @@ RouteParams route_params(const at::Tensor& logits, int64_t k, bool sigmoid, int6
   p.groups = (int)groups;
   p.topg = (int)topg;
   p.gbest = (int)std::min<int64_t>(std::max<int64_t>(1, k / topg), p.E / groups);
+  p.glanes = 1;
+  while (p.glanes * 2 * p.groups <= 32) p.glanes *= 2;
+  const int per = p.E / p.groups;
+  p.gstride = per + ((p.glanes - per) % 32 + 32) % 32;
   p.scaling = (float)scaling;
   p.sigmoid = sigmoid;
   p.renorm = renorm;
   return p;
 }
 
+// Calls f(type, experts per lane, whole aligned shares) for the shape.  The share of a lane is the smallest power of two
+// that gives 32 lanes all experts.
 template <typename F>
-void by_shape(at::ScalarType t, int E, F f) {
-  auto per = [&](auto v) {
-    const int epl = (E + 31) / 32;
-    if (epl <= 1) f(v, std::integral_constant<int, 1>{});
-    else if (epl <= 2) f(v, std::integral_constant<int, 2>{});
-    else if (epl <= 4) f(v, std::integral_constant<int, 4>{});
-    else if (epl <= 8) f(v, std::integral_constant<int, 8>{});
-    else f(v, std::integral_constant<int, 16>{});
+void by_shape(const at::Tensor& x, F f) {
+  const int E = (int)x.size(1);
+  auto per = [&](auto v, auto epl) {
+    constexpr int N = decltype(epl)::value;
+    const int bytes = std::min<int>(16, N * (int)sizeof(v));
+    const bool vec = N > 1 && E % N == 0 && (x.stride(0) * sizeof(v)) % bytes == 0 && (uintptr_t)x.data_ptr() % bytes == 0 &&
+                     ((int64_t)E * sizeof(v)) % bytes == 0;
+    if (vec) f(v, epl, std::true_type{});
+    else f(v, epl, std::false_type{});
   };
-  if (t == at::kFloat) per(float{});
-  else if (t == at::kBFloat16) per(__nv_bfloat16{});
-  else if (t == at::kHalf) per(__half{});
+  auto share = [&](auto v) {
+    const int epl = (E + 31) / 32;
+    if (epl <= 1) per(v, std::integral_constant<int, 1>{});
+    else if (epl <= 2) per(v, std::integral_constant<int, 2>{});
+    else if (epl <= 4) per(v, std::integral_constant<int, 4>{});
+    else if (epl <= 8) per(v, std::integral_constant<int, 8>{});
+    else per(v, std::integral_constant<int, 16>{});
+  };
+  const auto t = x.scalar_type();
+  if (t == at::kFloat) share(float{});
+  else if (t == at::kBFloat16) share(__nv_bfloat16{});
+  else if (t == at::kHalf) share(__half{});
   else TORCH_CHECK(false, "logits must be fp32, bf16 or fp16");
 }
 
@@ -398,20 +509,37 @@ std::vector<at::Tensor> moe_route_fwd(at::Tensor logits, int64_t k, bool sigmoid
   if (p.T == 0) return {weights, experts, at::zeros({p.E}, f32), at::zeros({p.E}, i32)};
   auto score_sum = at::empty({p.E}, f32), counts = at::empty({p.E}, i32);
   const int grid = std::min((p.T + kRouteWarps - 1) / kRouteWarps, num_sms() * 4);
-  auto part = at::empty({2, grid, p.E}, f32);
   p.bias = bias.has_value() ? bias->data_ptr<float>() : nullptr;
   p.weights = weights.data_ptr<float>();
   p.experts = experts.data_ptr<int>();
-  p.part = part.data_ptr<float>();
-  p.cpart = reinterpret_cast<int*>(p.part + (long long)grid * p.E);
-  const int smem = (kRouteWarps * p.E * (groups > topg ? 2 : 1) + p.E) * 4;
-  by_shape(x.scalar_type(), p.E, [&](auto v, auto epl) {
-    route_fwd_kernel<decltype(v), epl><<<grid, kRouteWarps * 32, smem, cur_stream()>>>(p);
+  at::Tensor part;
+  if (grid == 1) {  // one CTA sees every token: its sums are the result
+    p.part = score_sum.data_ptr<float>();
+    p.cpart = counts.data_ptr<int>();
+  } else {
+    part = at::empty({2, grid, p.E}, f32);
+    p.part = part.data_ptr<float>();
+    p.cpart = reinterpret_cast<int*>(p.part + (long long)grid * p.E);
+  }
+  by_shape(x, [&](auto v, auto epl, auto vec) {
+    constexpr int N = decltype(epl)::value;
+    const int smem = (2 * kRouteWarps * 32 * N + p.E + (groups > topg ? kRouteWarps * p.groups * p.gstride : 0)) * 4;
+    auto kern = route_fwd_kernel<decltype(v), N, decltype(vec)::value>;
+    if (smem > 48 * 1024) {
+      static bool done[kMaxDevices] = {};  // the limit belongs to the device's context
+      int dev = 0;
+      EMB_CUDA_CHECK(cudaGetDevice(&dev));
+      if (!done[dev]) EMB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
+      done[dev] = true;
+    }
+    kern<<<grid, kRouteWarps * 32, smem, cur_stream()>>>(p);
   });
-  route_join_kernel<<<(p.E + 31) / 32, 1024, 0, cur_stream()>>>(p.part, p.cpart, grid, p.E, score_sum.data_ptr<float>(),
-                                                                counts.data_ptr<int>());
   EMB_LAUNCH_CHECK();
-  count_launch(2);
+  if (grid > 1)
+    route_join_kernel<<<(p.E + 31) / 32, 1024, 0, cur_stream()>>>(p.part, p.cpart, grid, p.E, score_sum.data_ptr<float>(),
+                                                                  counts.data_ptr<int>());
+  EMB_LAUNCH_CHECK();
+  count_launch(grid > 1 ? 2 : 1);
   return {weights, experts, score_sum, counts};
 }
 
@@ -440,8 +568,8 @@ at::Tensor moe_route_bwd(at::Tensor logits, at::Tensor experts, c10::optional<at
   p.chosen = experts.data_ptr<int>();
   p.dlogits = dl.data_ptr();
   const int grid = std::min((p.T + kRouteWarps - 1) / kRouteWarps, num_sms() * 8);
-  by_shape(x.scalar_type(), p.E, [&](auto v, auto epl) {
-    route_bwd_kernel<decltype(v), epl><<<grid, kRouteWarps * 32, 0, cur_stream()>>>(p);
+  by_shape(x, [&](auto v, auto epl, auto vec) {
+    route_bwd_kernel<decltype(v), decltype(epl)::value, decltype(vec)::value><<<grid, kRouteWarps * 32, 0, cur_stream()>>>(p);
   });
   EMB_LAUNCH_CHECK();
   count_launch();
