@@ -37,7 +37,7 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr float kTiny = 1e-20f;
-constexpr int kRouteWarps = 8;
+constexpr int kRouteWarps = 16;
 constexpr int kMaxExperts = 512, kMaxTopk = 32, kMaxGroups = 32;
 
 struct RouteParams {
@@ -45,7 +45,8 @@ struct RouteParams {
   long long ld;  // elements between rows
   const float* bias;
   int T, E, k, groups, topg, gbest;
-  int glanes;   // lanes that value a group
+  int gwidth;   // lanes that hold a group, if groups are whole lanes of a power of two and gbest <= 2; else 0, and
+  int glanes;   // lanes that value a group from shared memory
   int gstride;  // words between groups in shared memory: the lanes of all groups hit different banks
   float scaling;
   int sigmoid, renorm;
@@ -143,7 +144,7 @@ __device__ __forceinline__ void sort_keys(unsigned* k) {
 }
 
 template <typename T, int EPL, bool VEC>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_fwd_kernel(RouteParams p) {
+__global__ void __launch_bounds__(kRouteWarps * 32, EPL <= 8 ? 2 : 1) route_fwd_kernel(RouteParams p) {
   // [warps, 32 EPL] keys, [warps, 32 EPL] scores (after the last token: score sums), [E] counts, [warps, groups, gstride]
   extern __shared__ __align__(16) unsigned s_mem[];
   constexpr int ROW = 32 * EPL;
@@ -156,22 +157,26 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_fwd_kernel(RouteParams
   __syncthreads();
   const bool by_group = p.groups > p.topg, by_logit = !p.bias && !by_group;
   const int per = p.E / p.groups;
-  float bias[EPL], acc[EPL];
-  int loc[EPL];  // expert's place in s_grp, and its group in the upper half
+  float bias[EPL], acc[EPL], next[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     const int e = lane * EPL + j;
     bias[j] = p.bias && e < p.E ? p.bias[e] : 0.f;
     acc[j] = 0.f;
-    const int g = e < p.E ? e / per : 0;
-    loc[j] = (g * p.gstride + e - g * per) | (g << 16);
   }
-  for (int t = blockIdx.x * kRouteWarps + warp; t < p.T; t += gridDim.x * kRouteWarps) {
+  const T* logits = reinterpret_cast<const T*>(p.logits);
+  const int step = gridDim.x * kRouteWarps;
+  int t = blockIdx.x * kRouteWarps + warp;
+  if (t < p.T) load_row<T, EPL, VEC>(logits + (long long)t * p.ld, p.E, lane, next);
+  for (; t < p.T; t += step) {
     float s[EPL];
     unsigned key[EPL];
+    float b1 = -INFINITY, b2 = -INFINITY;  // the lane's two largest choice values (groups of whole lanes)
     {
       float l[EPL];
-      load_row<T, EPL, VEC>(reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld, p.E, lane, l);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) l[j] = next[j];
+      if (t < p.T - step) load_row<T, EPL, VEC>(logits + (long long)(t + step) * p.ld, p.E, lane, next);
       if (p.sigmoid) {
         float sum = 0.f;
 #pragma unroll
@@ -197,10 +202,37 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_fwd_kernel(RouteParams
         const int e = lane * EPL + j;
         const float c = by_logit ? l[j] : l[j] > -INFINITY ? s[j] + bias[j] : -INFINITY;
         key[j] = e < p.E ? order_key(c) : 0u;
-        if (by_group && e < p.E) s_grp[loc[j] & 0xffff] = c;
+        if (by_group) {
+          if (p.gwidth) {
+            b2 = fmaxf(b2, fminf(b1, c == c ? c : -INFINITY));  // (NaN is passed over)
+            b1 = fmaxf(b1, c);
+          } else if (e < p.E) {
+            s_grp[e / per * p.gstride + e % per] = c;
+          }
+        }
       }
     }
-    if (by_group) {
+    if (by_group && p.gwidth) {
+      // the experts of a group are those of gwidth neighbouring lanes
+      for (int o = 1; o < p.gwidth; o <<= 1) {
+        const float o1 = __shfl_xor_sync(kFull, b1, o), o2 = __shfl_xor_sync(kFull, b2, o);
+        b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+        b1 = fmaxf(b1, o1);
+      }
+      unsigned gkey = lane * EPL < p.E && lane % p.gwidth == 0
+                          ? order_key(p.gbest == 2 && b2 > -INFINITY ? b1 + b2 : b1) : 0u;
+      unsigned kept = 0u;  // first lanes of the groups
+      for (int m = 0; m < p.topg; ++m) {
+        const unsigned top = __reduce_max_sync(kFull, gkey);
+        const unsigned at = __ballot_sync(kFull, gkey == top);
+        kept |= at & -at;
+        if (kept >> lane & 1u) gkey = 0u;
+      }
+      if (!((kept >> (lane & ~(p.gwidth - 1))) & 1u)) {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) key[j] = 0u;
+      }
+    } else if (by_group) {
       __syncwarp();
       // p.glanes lanes value a group, each from every glanes-th of its experts
       const int g = lane / p.glanes, part = lane % p.glanes;
@@ -209,7 +241,6 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_fwd_kernel(RouteParams
       bool any = false;
       const float* c = s_grp + (g < p.groups ? g : 0) * p.gstride;
       if (p.gbest <= 2) {
-        float b1 = -INFINITY, b2 = -INFINITY;  // the two largest (NaN is passed over)
         for (int i = part; i < per; i += p.glanes) {
           const float v = c[i];
           b2 = fmaxf(b2, fminf(b1, v == v ? v : -INFINITY));
@@ -262,8 +293,10 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_fwd_kernel(RouteParams
         if (lane == at) gkey = 0u;
       }
 #pragma unroll
-      for (int j = 0; j < EPL; ++j)
-        if (!((kept >> (loc[j] >> 16)) & 1u)) key[j] = 0u;
+      for (int j = 0; j < EPL; ++j) {
+        const int e = lane * EPL + j;
+        if (e < p.E && !((kept >> (e / per)) & 1u)) key[j] = 0u;
+      }
     }
     // keys and scores for the look-up of the chosen, then the lane's keys in falling order: a round takes the largest
     // of the lanes' first keys, and the lane that holds it moves up
@@ -273,14 +306,18 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_fwd_kernel(RouteParams
       s_val[lane * EPL + j] = s[j];
     }
     sort_keys<EPL>(key);
-    unsigned my_key = 0u;
-    int my_src = 0;
+    unsigned my_key = 0u, last = 0u;
+    int my_src = 0, skip = 0, from = -1, copies = 0;
     for (int r = 0; r < p.k; ++r) {
       const unsigned top = __reduce_max_sync(kFull, key[0]);
       const int src = __ffs(__ballot_sync(kFull, key[0] == top)) - 1;
+      copies = top == last && src == from ? copies + 1 : 0;  // equal keys of a lane come one after the other
+      last = top;
+      from = src;
       if (lane == r) {
         my_key = top;
         my_src = src;
+        skip = copies;
       }
       if (lane == src) {
 #pragma unroll
@@ -290,8 +327,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_fwd_kernel(RouteParams
     }
     __syncwarp();
     // lane r finds its expert: in lane my_src's share, the copy of my_key after those that earlier rounds took
-    const unsigned same = __match_any_sync(kFull, my_key) & __match_any_sync(kFull, my_src) & ((1u << lane) - 1u);
-    int skip = __popc(same), mine = 0;
+    int mine = 0;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
       if (s_key[my_src * EPL + j] == my_key) {
@@ -331,6 +367,7 @@ __global__ void __launch_bounds__(1024) route_join_kernel(const float* __restric
   float v = 0.f;
   int c = 0;
   if (e < E) {
+#pragma unroll 8
     for (int b = slice; b < blocks; b += 32) {
       v += part[(long long)b * E + e];
       c += cpart[(long long)b * E + e];
@@ -361,24 +398,34 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_bwd_kernel(RouteParams
     row[e] = 0.f;
   }
   __syncwarp();
-  for (int t = blockIdx.x * kRouteWarps + warp; t < p.T; t += gridDim.x * kRouteWarps) {
-    const T* logits = reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld;
-    float l[EPL], s[EPL];
-    load_row<T, EPL, VEC>(logits, p.E, lane, l);
-    // lane r has the r-th chosen expert: its gradient and its score
-    float a = 0.f, sr = 0.f, lr = -INFINITY;
-    int er = 0;
+  // lane r has the r-th chosen expert: its gradient and its score.  The next token's inputs are fetched ahead.
+  float next[EPL], next_a = 0.f;
+  int next_e = 0;
+  auto fetch = [&](int t) {
+    load_row<T, EPL, VEC>(reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld, p.E, lane, next);
     if (lane < p.k) {
-      er = p.chosen[(long long)t * p.k + lane];
-      lr = (float)logits[er];
-      if (p.dweights) a = p.dweights[(long long)t * p.k + lane] * p.scaling;
+      next_e = p.chosen[(long long)t * p.k + lane];
+      if (p.dweights) next_a = p.dweights[(long long)t * p.k + lane];
     }
+  };
+  const int step = gridDim.x * kRouteWarps;
+  int t = blockIdx.x * kRouteWarps + warp;
+  if (t < p.T) fetch(t);
+  for (; t < p.T; t += step) {
+    float l[EPL], s[EPL];
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) l[j] = next[j];
+    const float a = next_a * p.scaling;
+    const int er = next_e;
+    const float lr = lane < p.k ? (float)(reinterpret_cast<const T*>(p.logits) + (long long)t * p.ld)[er] : -INFINITY;
+    if (t < p.T - step) fetch(t + step);
+    float sr = 0.f;
     float norm = 1.f, dsum = 0.f;  // dsum: s (1 - s) for the sigmoid is kept in l
     if (p.sigmoid) {
       float total = 0.f;
 #pragma unroll
       for (int j = 0; j < EPL; ++j) {
-        const float x = expf(-fabsf(l[j])), y = __frcp_rn(1.f + x);
+        const float x = expf(-fabsf(l[j])), y = __fdividef(1.f, 1.f + x);
         s[j] = l[j] >= 0.f ? y : x * y;
         l[j] = x * y * y;  // s (1 - s), without the difference
         total += s[j];
@@ -465,8 +512,14 @@ RouteParams route_params(const at::Tensor& logits, int64_t k, bool sigmoid, int6
   return p;
 }
 
-// Calls f(type, experts per lane, whole aligned shares) for the shape.  The share of a lane is the smallest power of two
-// that gives 32 lanes all experts.
+// Experts of a lane: the smallest power of two that gives 32 lanes all experts.
+int lane_share(int E) {
+  int n = 1;
+  while (32 * n < E) n *= 2;
+  return n;
+}
+
+// Calls f(type, experts per lane, whole aligned shares) for the shape.
 template <typename F>
 void by_shape(const at::Tensor& x, F f) {
   const int E = (int)x.size(1);
@@ -479,12 +532,13 @@ void by_shape(const at::Tensor& x, F f) {
     else f(v, epl, std::false_type{});
   };
   auto share = [&](auto v) {
-    const int epl = (E + 31) / 32;
-    if (epl <= 1) per(v, std::integral_constant<int, 1>{});
-    else if (epl <= 2) per(v, std::integral_constant<int, 2>{});
-    else if (epl <= 4) per(v, std::integral_constant<int, 4>{});
-    else if (epl <= 8) per(v, std::integral_constant<int, 8>{});
-    else per(v, std::integral_constant<int, 16>{});
+    switch (lane_share(E)) {
+      case 1: return per(v, std::integral_constant<int, 1>{});
+      case 2: return per(v, std::integral_constant<int, 2>{});
+      case 4: return per(v, std::integral_constant<int, 4>{});
+      case 8: return per(v, std::integral_constant<int, 8>{});
+      default: return per(v, std::integral_constant<int, 16>{});
+    }
   };
   const auto t = x.scalar_type();
   if (t == at::kFloat) share(float{});
@@ -508,7 +562,10 @@ std::vector<at::Tensor> moe_route_fwd(at::Tensor logits, int64_t k, bool sigmoid
   auto weights = at::empty({p.T, k}, f32), experts = at::empty({p.T, k}, i32);
   if (p.T == 0) return {weights, experts, at::zeros({p.E}, f32), at::zeros({p.E}, i32)};
   auto score_sum = at::empty({p.E}, f32), counts = at::empty({p.E}, i32);
-  const int grid = std::min((p.T + kRouteWarps - 1) / kRouteWarps, num_sms() * 4);
+  const int epl = lane_share(p.E), width = p.E / p.groups / epl;
+  p.gwidth = p.gbest <= 2 && (p.E / p.groups) % epl == 0 && (width & (width - 1)) == 0 ? width : 0;
+  // (twice the resident CTAs would give a second, partial wave)
+  const int grid = std::min((p.T + kRouteWarps - 1) / kRouteWarps, num_sms() * (epl <= 8 ? 2 : 1));
   p.bias = bias.has_value() ? bias->data_ptr<float>() : nullptr;
   p.weights = weights.data_ptr<float>();
   p.experts = experts.data_ptr<int>();
@@ -523,7 +580,8 @@ std::vector<at::Tensor> moe_route_fwd(at::Tensor logits, int64_t k, bool sigmoid
   }
   by_shape(x, [&](auto v, auto epl, auto vec) {
     constexpr int N = decltype(epl)::value;
-    const int smem = (2 * kRouteWarps * 32 * N + p.E + (groups > topg ? kRouteWarps * p.groups * p.gstride : 0)) * 4;
+    const int smem = (2 * kRouteWarps * 32 * N + p.E +
+                      (groups > topg && !p.gwidth ? kRouteWarps * p.groups * p.gstride : 0)) * 4;
     auto kern = route_fwd_kernel<decltype(v), N, decltype(vec)::value>;
     if (smem > 48 * 1024) {
       static bool done[kMaxDevices] = {};  // the limit belongs to the device's context
@@ -567,7 +625,7 @@ at::Tensor moe_route_bwd(at::Tensor logits, at::Tensor experts, c10::optional<at
   }
   p.chosen = experts.data_ptr<int>();
   p.dlogits = dl.data_ptr();
-  const int grid = std::min((p.T + kRouteWarps - 1) / kRouteWarps, num_sms() * 8);
+  const int grid = std::min((p.T + kRouteWarps - 1) / kRouteWarps, num_sms() * 4);
   by_shape(x, [&](auto v, auto epl, auto vec) {
     route_bwd_kernel<decltype(v), decltype(epl)::value, decltype(vec)::value><<<grid, kRouteWarps * 32, 0, cur_stream()>>>(p);
   });
