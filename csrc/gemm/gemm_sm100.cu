@@ -155,6 +155,7 @@ struct Params {
   int a_mn, b_mn;  // operand majorness
   int* err;
   int split_tail;  // 2-SM kernel: run the last partial wave as 256 x 128 half tiles when they fit in one wave
+  int raster;      // 2-SM kernel: width of the bands in which tiles are walked (0: no bands)
   int m_fast;      // measurement only (EMB_GEMM_RASTER=m): m blocks vary fastest whatever the shape
   int no_store;    // 2-SM kernel, measurement only: read the accumulators but write no output
   int c_tma;       // 2-SM kernel: C is written (or add-reduced) through the tensor map tmC, one 32-row block per
@@ -599,11 +600,20 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
   const int my_chunk = AG ? p.my_slot : 0;
   const int mt_per_chunk = AG ? p.rows_per_rank / BM : 1;
   const bool n_fast = AG || (tiles_n < tiles_m && !p.m_fast);
+  // With p.raster the faster dimension is cut into bands of that many tiles, walked one after the other: the 74 tiles
+  // in flight then form a block of about 8 x 9, the band's panels stay in L2 and the long operand is streamed once per
+  // band.  (8192 x 16384 x 4096: 1.58 -> 0.6 GB read from DRAM.)
+  const int fast = n_fast ? tiles_n : tiles_m, slow = n_fast ? tiles_m : tiles_n;
+  const int band = !AG && p.raster > 0 && p.raster < fast ? p.raster : fast;
+  auto tile_fs = [&](int t, bool want_fast) -> int {
+    const int b = t / (band * slow), r = t - b * band * slow, width = min(band, fast - b * band);
+    return want_fast ? b * band + r % width : r / width;
+  };
   auto tile_m = [&](int t) -> int {
     if (AG) return (t / tiles_n + my_chunk * mt_per_chunk) % tiles_m;
-    return n_fast ? t / tiles_n : t % tiles_m;
+    return tile_fs(t, !n_fast);
   };
-  auto tile_n = [&](int t) -> int { return n_fast ? t % tiles_n : t / tiles_m; };
+  auto tile_n = [&](int t) -> int { return AG ? t % tiles_n : tile_fs(t, n_fast); };
   // Tail split (not with the all-gather prologue): when the tiles of the last, partial wave could run as twice
   // as many 256 x 128 halves in one wave, they do - the last wave then takes half as long (4096 x 4096
   // outputs: 256 tiles on 74 clusters = 3 full waves + 34 tiles -> 3.5 wave-times instead of 4).  Work unit u
@@ -1130,6 +1140,11 @@ static void launch(int bk, const CUtensorMap& tA, const CUtensorMap& tB, const C
 }
 }  // namespace gk2
 
+// Width of the bands in which a large product walks its tiles: the band's panels (256 x K bf16 each) take about 32 MB of
+// L2, in 8 to 16 tiles.  Measured at 8192 x 16384 x 4096, TFLOP/s with bands of 4 / 8 / 16 tiles and without: logits
+// (K = 4096) 1457 / 1524 / 1562 / 1475, dx (K = 16384) 1504 / 1526 / 1498 / 1498, dw (K = 8192) 1502 / 1526 / 1488 / 1488.
+static int raster_band(int64_t K) { return (int)std::min<int64_t>(16, std::max<int64_t>(8, 65536 / K)); }
+
 static bool ok_2d(const at::Tensor& t) {
   return t.dim() == 2 && t.stride(1) == 1 && t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) == 0;
 }
@@ -1185,6 +1200,10 @@ at::Tensor gemm_tc(at::Tensor a, at::Tensor b, bool trans_a, bool trans_b, c10::
   CUtensorMap tB = b_mn ? make_map(b.data_ptr(), K, N, b.stride(0), 64, 64) : make_map(b.data_ptr(), N, K, b.stride(0), 64, BN);
   Params p{};
   p.m_fast = raster_m_fast();
+  if (variant == 16) {  // auto, with the tiles walked in bands
+    p.raster = raster_band(K);
+    variant = 0;
+  }
   p.C = C.data_ptr();
   p.M = (int)M;
   p.N = (int)N;
@@ -1324,6 +1343,7 @@ void linear_ce_gemm(const at::Tensor& x, const at::Tensor& w, const CeArgs& ce, 
   p.N = (int)N;
   p.K = (int)K;
   p.err = err_flag();
+  p.raster = raster_band(K);
   p.ce = ce;
   if (grad) {
     p.C = out.data_ptr();

@@ -92,6 +92,7 @@ CeArgs ce_args(const at::Tensor& labels, int64_t col0, int64_t vocab, int64_t ig
 
 // Columns of a piece of the vocabulary in the backward pass: as many as keep its bf16 gradient within 256 MiB.
 constexpr int64_t kPieceBytes = 256ll << 20;
+constexpr int kBands = 16;  // gemm_tc: choose the kernel by size and walk the tiles in bands
 
 }  // namespace
 
@@ -176,11 +177,11 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
         gemm_split_k(Pi, wi, parts.narrow(0, part, shares(n)));
         part += shares(n);
       } else {
-        gemm_tc(Pi, wi, false, false, pieces > 1 ? parts[0] : dx, i > 0, 0);
+        gemm_tc(Pi, wi, false, false, pieces > 1 ? parts[0] : dx, i > 0, kBands);
       }
     }
-    if (dw_accum.has_value()) gemm_tc(Pi, xr, true, false, dw_accum->narrow(0, v0, n), true, 0);
-    else if (want_dw) gemm_tc(Pi, xr, true, false, dw.narrow(0, v0, n), false, 0);
+    if (dw_accum.has_value()) gemm_tc(Pi, xr, true, false, dw_accum->narrow(0, v0, n), true, kBands);
+    else if (want_dw) gemm_tc(Pi, xr, true, false, dw.narrow(0, v0, n), false, kBands);
   }
   if (parts.defined()) {
     const int64_t vecs = T * H / 4;
