@@ -397,9 +397,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         TMEM_LD_32(taddr, r);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         const int col0 = n0 + c * 32;
+        if constexpr (EPI == kCeGrad) ce_grad_chunk(ce_row, r, col0);  // by the whole warp
         if (!row_ok || col0 >= p.N) continue;
         const int ncols = min(32, p.N - col0);
-        if constexpr (EPI == kCeGrad) ce_grad_chunk(ce_row, r, col0);
         if (p.out_fp32) {
           float* dst = reinterpret_cast<float*>(p.C) + ti.c_off + (size_t)row * p.ldc + col0;
           if (ncols == 32 && ((reinterpret_cast<uintptr_t>(dst) & 15) == 0)) {
@@ -901,9 +901,9 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
         TMEM_LD_32(taddr, r);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         const int col0 = n0 + c * 32;
+        if constexpr (EPI == kCeGrad) ce_grad_chunk(ce_row, r, col0);  // by the whole warp
         if (!row_ok || col0 >= p.N || p.no_store) continue;
         const int ncols = min(32, p.N - col0);
-        if constexpr (EPI == kCeGrad) ce_grad_chunk(ce_row, r, col0);
         void* gdst;
         if (p.scatter) {
           // fused reduce-scatter: this partial row chunk goes straight to its owner's staging slot (peer memory
