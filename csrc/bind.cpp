@@ -28,6 +28,11 @@ std::vector<torch::Tensor> heads_bwd(torch::Tensor dy, c10::optional<torch::Tens
                                      c10::optional<torch::Tensor> wq, c10::optional<torch::Tensor> wk, double eps,
                                      c10::optional<torch::Tensor> dwq_accum, c10::optional<torch::Tensor> dwk_accum);
 int64_t heads_error_flag();
+torch::Tensor heads(torch::Tensor qkv, c10::optional<torch::Tensor> wq, c10::optional<torch::Tensor> wk, torch::Tensor cosv,
+                    torch::Tensor sinv, int64_t nq, int64_t nk, double eps, bool interleaved);
+std::vector<torch::Tensor> moe_route(torch::Tensor logits, c10::optional<torch::Tensor> bias, int64_t k, bool sigmoid,
+                                     int64_t groups, int64_t topg, bool renorm, double scaling);
+torch::Tensor linear_ce(torch::Tensor x, torch::Tensor w, torch::Tensor labels, int64_t ignore, int64_t piece);
 torch::Tensor ce_local_max(torch::Tensor logits);
 torch::Tensor ce_local_stats(torch::Tensor logits, torch::Tensor labels, torch::Tensor lmax, int64_t vstart);
 torch::Tensor ce_bwd(torch::Tensor logits, torch::Tensor labels, torch::Tensor lmax, torch::Tensor sumexp,
@@ -121,6 +126,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu_fwd", &swiglu_fwd);
   m.def("swiglu_bwd", &swiglu_bwd);
   m.def("rope_fwd", &rope_fwd);
+  m.def("heads", &heads);
+  m.def("moe_route", &moe_route);
+  m.def("linear_ce", &linear_ce);
   m.def("heads_fwd", &heads_fwd);
   m.def("heads_bwd", &heads_bwd);
   m.def("heads_error_flag", &heads_error_flag);

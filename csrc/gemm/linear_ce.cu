@@ -15,13 +15,22 @@ namespace emb {
 namespace {
 
 // Joins the tiles' statistics of a row: 32 rows a CTA, 32 slices of the tiles, in a fixed order.
-__global__ void __launch_bounds__(1024) ce_join_kernel(CeArgs ce, int T, int tiles, int V, bool raw,
-                                                       float* __restrict__ out, float* __restrict__ out_top,
-                                                       float* __restrict__ out_sum) {
+//
+// The label's logit is taken again as an fp32 dot product of x's row and w's.  Tensor cores cut their sums off towards
+// zero at every step of K (3.8e-6 of a logit at K = 4096, the library's product alike), which the loss of a token with a
+// large logit shows; with the label's own term exchanged in the sum and in the difference the loss of such a token
+// depends on the exact value, and the rest of the sum on small logits (4096 tokens of which some are certain: relative
+// error of the losses 1.9e-6 -> 0.75e-6).  `out_sum` stays the sum that the gradient's logits belong to.
+__global__ void __launch_bounds__(1024) ce_join_kernel(CeArgs ce, const __nv_bfloat16* __restrict__ x, int64_t ldx,
+                                                       const __nv_bfloat16* __restrict__ w, int64_t ldw, int H, int T,
+                                                       int tiles, int V, bool raw, float* __restrict__ out,
+                                                       float* __restrict__ out_top, float* __restrict__ out_sum,
+                                                       float* __restrict__ out_loss_sum) {
   __shared__ float sm[32][33], ss[32][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f;
   if (row < T) {
+#pragma unroll 4
     for (int i = slice; i < tiles; i += 32) {
       const float2 v = ce.part[(size_t)i * T + row];
       const float top = fmaxf(m, v.x), base = top == -INFINITY ? 0.f : top;
@@ -31,26 +40,46 @@ __global__ void __launch_bounds__(1024) ce_join_kernel(CeArgs ce, int T, int til
   }
   sm[slice][lane] = m;
   ss[slice][lane] = s;
+  // warp `slice` finishes row t
+  const int t = blockIdx.x * 32 + slice;
+  int64_t label = -1;
+  if (t < T) label = ce.labels[t];
+  const bool own = t < T && ce_counts(ce, label) && label >= ce.col0 && label < ce.col0 + V;
+  float dot = 0.f;
+  if (own) {
+    const uint4* a = reinterpret_cast<const uint4*>(x + t * ldx);
+    const uint4* b = reinterpret_cast<const uint4*>(w + (label - ce.col0) * ldw);
+#pragma unroll 4
+    for (int i = lane; i < H / 8; i += 32) {
+      float f[8], g[8];
+      unpack8(a[i], f);
+      unpack8(b[i], g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot += f[j] * g[j];
+    }
+  }
+  dot = warp_sum(dot);
   __syncthreads();
-  m = sm[lane][slice];  // slices of row blockIdx.x * 32 + slice
+  if (t >= T) return;
+  m = sm[lane][slice];
   s = ss[lane][slice];
   const float top = warp_max(m), base = top == -INFINITY ? 0.f : top;
   s = warp_sum(s * __expf(m - base));
-  const int t = blockIdx.x * 32 + slice;
-  if (lane != 0 || t >= T) return;
-  const int64_t label = ce.labels[t];
-  const bool counts = ce_counts(ce, label);
-  const bool own = counts && label >= ce.col0 && label < ce.col0 + V;
+  if (lane != 0) return;
   out_top[t] = top;
   out_sum[t] = s;
-  // a rank's share of the vocabulary leaves the label's logit, for the caller to join the ranks
-  out[t] = !own ? 0.f : raw ? ce.target[t] : logf(s) + (top - ce.target[t]);
+  float z = s;
+  if (own) z = fmaxf(s - __expf(ce.target[t] - top), 0.f) + __expf(dot - top);
+  // a rank's share of the vocabulary leaves the label's logit and the sum that belongs to it, for the caller to join
+  if (raw) out_loss_sum[t] = z;
+  out[t] = !own ? 0.f : raw ? dot : logf(z) + (top - dot);
 }
 
 // out[i] = bf16(sum over the n fp32 parts, in order)
 __global__ void parts_sum_kernel(const float4* __restrict__ parts, int n, int64_t vecs, __nv_bfloat16* __restrict__ out) {
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < vecs; i += (int64_t)gridDim.x * blockDim.x) {
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
     for (int p = 0; p < n; ++p) {
       const float4 v = parts[p * vecs + i];
       a.x += v.x;
@@ -64,13 +93,15 @@ __global__ void parts_sum_kernel(const float4* __restrict__ parts, int n, int64_
 }
 
 void check_ce(const at::Tensor& x, const at::Tensor& w, const at::Tensor& labels) {
+  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && x.size(1) % 8 == 0 && x.size(1) > 0 &&
+                        w.size(0) > 0, "x must be [T, H] and w [V, H] with H a multiple of 8");
+  TORCH_CHECK_VALUE(x.scalar_type() == w.scalar_type(), "x and w must have the same type");
+  TORCH_CHECK_VALUE(labels.scalar_type() == at::kLong && labels.dim() == 1 && labels.size(0) == x.size(0),
+                    "labels must be int64 [T]");
   TORCH_CHECK(x.is_cuda() && w.is_cuda() && labels.is_cuda() && x.device() == w.device() && x.device() == labels.device(),
               "x, w and labels must be on one CUDA device");
-  TORCH_CHECK(x.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16, "x and w must be bf16");
-  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && x.size(1) % 8 == 0 && x.size(1) > 0,
-              "x [T, H] and w [V, H] with H a multiple of 8");
-  TORCH_CHECK(labels.scalar_type() == at::kLong && labels.dim() == 1 && labels.size(0) == x.size(0) && labels.is_contiguous(),
-              "labels must be a contiguous int64 [T]");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16, "x and w must be bf16");
+  TORCH_CHECK(labels.is_contiguous(), "labels must be contiguous");
   TORCH_CHECK(x.size(0) < (1ll << 31) - 256 && w.size(0) < (1ll << 31) - 256, "too many rows");
 }
 
@@ -96,8 +127,8 @@ constexpr int kBands = 16;  // gemm_tc: choose the kernel by size and walk the t
 
 }  // namespace
 
-// {loss [T], max [T], sum exp(z - max) [T]} for a whole vocabulary; with `raw`, of the columns [col0, col0 + V) that this
-// rank holds of `vocab`, and the label's logit (0 where another rank holds it) in place of the loss.
+// {loss [T], max [T], sum exp(z - max) [T]} for a whole vocabulary; with `raw`, {label's logit (0 where another rank holds
+// it), max, sum, sum with the label's logit exchanged} of the columns [col0, col0 + V) that this rank holds of `vocab`.
 std::vector<at::Tensor> linear_ce_fwd(at::Tensor x, at::Tensor w, at::Tensor labels, int64_t col0, int64_t vocab,
                                       int64_t ignore, bool raw) {
   check_ce(x, w, labels);
@@ -105,17 +136,20 @@ std::vector<at::Tensor> linear_ce_fwd(at::Tensor x, at::Tensor w, at::Tensor lab
   const int64_t T = x.size(0), V = w.size(0);
   TORCH_CHECK(V > 0 && col0 >= 0 && col0 + V <= vocab && (raw || V == vocab), "columns outside the vocabulary");
   auto f32 = x.options().dtype(at::kFloat);
-  auto out = at::empty({3, T}, f32);
+  auto out = at::empty({raw ? 4 : 3, T}, f32);
   if (T == 0) return out.unbind(0);
   const int64_t tiles = (V + 255) / 256;
   auto part = at::empty({tiles, T, 2}, f32), target = at::empty({T}, f32);
   CeArgs ce = ce_args(labels, col0, vocab, ignore);
   ce.part = reinterpret_cast<float2*>(part.data_ptr<float>());
   ce.target = target.data_ptr<float>();
-  linear_ce_gemm(tma_rows(x), tma_rows(w), ce, false, at::Tensor());
+  auto xr = tma_rows(x), wr = tma_rows(w);
+  linear_ce_gemm(xr, wr, ce, false, at::Tensor());
   float* o = out.data_ptr<float>();
-  ce_join_kernel<<<(int)((T + 31) / 32), 1024, 0, cur_stream()>>>(ce, (int)T, (int)tiles, (int)V, raw, o, o + T,
-                                                                  o + 2 * T);
+  ce_join_kernel<<<(int)((T + 31) / 32), 1024, 0, cur_stream()>>>(
+      ce, reinterpret_cast<const __nv_bfloat16*>(xr.data_ptr()), xr.stride(0),
+      reinterpret_cast<const __nv_bfloat16*>(wr.data_ptr()), wr.stride(0), (int)x.size(1), (int)T, (int)tiles, (int)V, raw, o,
+      o + T, o + 2 * T, raw ? o + 3 * T : nullptr);
   EMB_LAUNCH_CHECK();
   count_launch();
   return out.unbind(0);

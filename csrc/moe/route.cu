@@ -477,18 +477,20 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_bwd_kernel(RouteParams
 }
 
 void check_route(const at::Tensor& logits, int64_t k, int64_t groups, int64_t topg, const c10::optional<at::Tensor>& bias) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be a CUDA tensor [tokens, experts]");
+  TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
+  TORCH_CHECK_VALUE(logits.dim() == 2, "logits must be [tokens, experts]");
   const int64_t E = logits.size(1);
-  TORCH_CHECK(E >= 1 && E <= kMaxExperts, "1 to ", kMaxExperts, " experts are supported");
-  TORCH_CHECK(k >= 1 && k <= E && k <= kMaxTopk, "k must be in 1..min(experts, ", kMaxTopk, ")");
-  TORCH_CHECK(groups >= 1 && groups <= kMaxGroups && E % groups == 0, "experts must divide into at most ", kMaxGroups,
-              " groups");
-  TORCH_CHECK(topg >= 1 && topg <= groups && topg * (E / groups) >= k, "the kept groups must hold k experts");
+  TORCH_CHECK_VALUE(E >= 1 && E <= kMaxExperts, "1 to ", kMaxExperts, " experts are supported");
+  TORCH_CHECK_VALUE(k >= 1 && k <= E && k <= kMaxTopk, "k must be in 1..min(experts, ", kMaxTopk, ")");
+  TORCH_CHECK_VALUE(groups >= 1 && groups <= kMaxGroups && E % groups == 0, "experts must divide into at most ", kMaxGroups,
+                    " groups");
+  TORCH_CHECK_VALUE(topg >= 1 && topg <= groups && topg * (E / groups) >= k, "the kept groups must hold k experts");
   TORCH_CHECK(logits.size(0) < (1ll << 31) - (1 << 20), "too many tokens in one call");
-  if (bias.has_value())
-    TORCH_CHECK(bias->is_cuda() && bias->device() == logits.device() && bias->scalar_type() == at::kFloat &&
-                    bias->dim() == 1 && bias->size(0) == E && bias->is_contiguous(),
-                "bias must be a contiguous fp32 [experts] tensor on the device of logits");
+  if (bias.has_value()) {
+    TORCH_CHECK_VALUE(bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == E, "bias must be fp32 [experts]");
+    TORCH_CHECK(bias->is_cuda() && bias->device() == logits.device() && bias->is_contiguous(),
+                "bias must be contiguous and on the device of logits");
+  }
 }
 
 RouteParams route_params(const at::Tensor& logits, int64_t k, bool sigmoid, int64_t groups, int64_t topg, bool renorm,

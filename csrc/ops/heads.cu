@@ -746,9 +746,9 @@ void pick_shape(const HeadParams& p, int grid, bool vec, bool inter, bool norm, 
 void check_table(const at::Tensor& t, const at::Tensor& qkv, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == qkv.device() && t.scalar_type() == at::kFloat, name,
               " must be an fp32 tensor on the device of qkv");
-  TORCH_CHECK(t.dim() == 2 || t.dim() == 3, name, " must be [s, r/2] or [s, b, r/2]");
-  TORCH_CHECK(t.size(0) == qkv.size(0) && (t.dim() == 2 || t.size(1) == qkv.size(1)), name,
-              " must have a row for every position of qkv");
+  TORCH_CHECK_VALUE(t.dim() == 2 || t.dim() == 3, name, " must be [s, r/2] or [s, b, r/2]");
+  TORCH_CHECK_VALUE(t.size(0) == qkv.size(0) && (t.dim() == 2 || t.size(1) == qkv.size(1)), name,
+                    " must have a row for every position of qkv");
   TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
 }
 
@@ -761,14 +761,14 @@ at::Tensor inner_contiguous(const at::Tensor& t) {
 
 // Fills the parameters that forward and backward share; returns whether rows allow 8-channel vectors.
 bool set_up(HeadParams& p, const at::Tensor& t, const at::Tensor& cosv, const at::Tensor& sinv, int64_t nq, int64_t nk) {
-  TORCH_CHECK(t.dim() == 5, "qkv must be [s, b, G, slots, d]");
+  TORCH_CHECK_VALUE(t.dim() == 5, "qkv must be [s, b, groups, slots, d]");
   const int64_t s = t.size(0), b = t.size(1), G = t.size(2), S = t.size(3), d = t.size(4);
-  TORCH_CHECK(nq >= 0 && nk >= 0 && nq + nk <= S, "more query and key heads than slots in a group");
+  TORCH_CHECK_VALUE(nq >= 0 && nk >= 0 && nq + nk <= S, "more query and key heads than slots in a group");
   check_table(cosv, t, "cos");
   check_table(sinv, t, "sin");
-  TORCH_CHECK(cosv.sizes() == sinv.sizes(), "cos and sin must have the same shape");
+  TORCH_CHECK_VALUE(cosv.sizes() == sinv.sizes(), "cos and sin must have the same shape");
   const int64_t r = 2 * cosv.size(-1);
-  TORCH_CHECK(d <= 512 && d % 2 == 0 && r <= d, "head size must be even, at most 512, and hold the turned channels");
+  TORCH_CHECK_VALUE(d <= 512 && d % 2 == 0 && r <= d, "head size must be even, at most 512, and hold the turned channels");
   TORCH_CHECK(s * b * G * S < (1ll << 30), "too many heads in one call");
   p.cosv = cosv.data_ptr<float>();
   p.sinv = sinv.data_ptr<float>();
@@ -892,9 +892,10 @@ void by_type(at::ScalarType t, F f) {
 constexpr int kHeadWaves = 8;
 
 void check_weights(const c10::optional<at::Tensor>& w, const at::Tensor& t, const char* name) {
-  TORCH_CHECK(w.has_value() && w->is_cuda() && w->device() == t.device() && w->scalar_type() == t.scalar_type() &&
-                  w->dim() == 1 && w->size(0) == t.size(4) && w->is_contiguous(),
-              name, " must be a contiguous [d] tensor of qkv's type and device");
+  TORCH_CHECK_VALUE(w.has_value() && w->scalar_type() == t.scalar_type() && w->dim() == 1 && w->size(0) == t.size(4), name,
+                    " must be [d] of qkv's type");
+  TORCH_CHECK(w->is_cuda() && w->device() == t.device() && w->is_contiguous(), name,
+              " must be contiguous and on the device of qkv");
 }
 
 }  // namespace

@@ -456,6 +456,8 @@ def qk_norm_rope_qkv(qkv, q_weight, k_weight, cos, sin, eps, interleaved: bool =
     in fp32 into ``main_grad`` where the parameters have one.  Tables and layouts as for :func:`rope_qkv`."""
     if qkv.dim() == 5 and qkv.shape[3] < 3:
         raise ValueError("a group needs at least one query head, the key head and the value head")
+    if use_native(qkv) and qkv.dim() == 5 and not hasattr(q_weight, "main_grad") and not hasattr(k_weight, "main_grad"):
+        return ext().heads(qkv, q_weight, k_weight, cos, sin, qkv.shape[3] - 2, 1, eps, interleaved)
     _check_heads(qkv, cos, sin, qkv.shape[3] - 1 if qkv.dim() == 5 else 0)
     for n, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if tuple(w.shape) != (qkv.shape[-1],) or w.dtype != qkv.dtype:
@@ -554,23 +556,21 @@ def attention(qkv, hpg):
 
 # ------------------------------------------------------------------------------------------ MoE router
 class MoERouteFn(torch.autograd.Function):
-    """(weights [T, k], score_sum [E], experts [T, k], counts [E]) of :func:`moe_route`."""
+    """:func:`moe_route` on the host (CUDA tensors take the extension's node)."""
 
     @staticmethod
     def forward(ctx, logits, bias, k, sigmoid, groups, topg, renorm, scaling):
-        fwd = ext().moe_route_fwd if use_native(logits) else ref.moe_route_fwd
-        weights, experts, score_sum, counts = fwd(logits, k, sigmoid, bias, groups, topg, renorm, scaling)
+        weights, experts, score_sum, counts = ref.moe_route_fwd(logits, k, sigmoid, bias, groups, topg, renorm, scaling)
         ctx.save_for_backward(logits, experts)
         ctx.rest = (sigmoid, renorm, scaling)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(experts, counts)
-        return weights, score_sum, experts, counts
+        return weights, experts, score_sum, counts
 
     @staticmethod
-    def backward(ctx, dweights, dscore, _experts, _counts):
+    def backward(ctx, dweights, _experts, dscore, _counts):
         logits, experts = ctx.saved_tensors
-        bwd = ext().moe_route_bwd if use_native(logits) else ref.moe_route_bwd
-        return (bwd(logits, experts, dweights, dscore, *ctx.rest),) + (None,) * 7
+        return (ref.moe_route_bwd(logits, experts, dweights, dscore, *ctx.rest),) + (None,) * 7
 
 
 def moe_route(logits, k: int, score_function: str = "softmax", bias: Optional[torch.Tensor] = None, num_groups: int = 1,
@@ -586,11 +586,14 @@ def moe_route(logits, k: int, score_function: str = "softmax", bias: Optional[to
     times ``scaling``; ``experts`` [T, k] int32; ``score_sum`` [E] is the sum over the tokens of the scores (sigmoid
     scores normalised over the experts) for a load-balancing loss; ``counts`` [E] int32 the tokens of each expert.
     ``weights`` and ``score_sum`` carry gradients to ``logits``."""
+    if score_function not in ("softmax", "sigmoid"):
+        raise ValueError(f"score_function must be softmax or sigmoid, got {score_function!r}")
+    sigmoid = score_function == "sigmoid"
+    if use_native(logits):  # (the extension checks the arguments)
+        return tuple(ext().moe_route(logits, bias, k, sigmoid, num_groups, group_topk, renormalize, scaling))
     if logits.dim() != 2:
         raise ValueError(f"logits must be [tokens, experts], got {tuple(logits.shape)}")
     E = logits.shape[1]
-    if score_function not in ("softmax", "sigmoid"):
-        raise ValueError(f"score_function must be softmax or sigmoid, got {score_function!r}")
     if not (1 <= E <= 512 and 1 <= k <= min(E, 32)):
         raise ValueError(f"1 to 512 experts and 1 <= k <= min(experts, 32) are supported, got {E} and k={k}")
     if not (1 <= num_groups <= 32) or E % num_groups:
@@ -599,9 +602,7 @@ def moe_route(logits, k: int, score_function: str = "softmax", bias: Optional[to
         raise ValueError(f"{group_topk} of {num_groups} groups of {E // num_groups} do not hold k={k} experts")
     if bias is not None and (tuple(bias.shape) != (E,) or bias.dtype != torch.float32):
         raise ValueError(f"bias must be fp32 [{E}], got {tuple(bias.shape)} {bias.dtype}")
-    weights, score_sum, experts, counts = MoERouteFn.apply(logits, bias, k, score_function == "sigmoid", num_groups,
-                                                           group_topk, renormalize, scaling)
-    return weights, experts, score_sum, counts
+    return MoERouteFn.apply(logits, bias, k, sigmoid, num_groups, group_topk, renormalize, scaling)
 
 
 # ------------------------------------------------------------------------------------------ vocab-parallel CE
@@ -678,17 +679,18 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         if mode is None:
             loss, m, total = fwd(xf, w, labels, vocab_start, vocab, ignore_index, False)
         else:
-            target, top, total = fwd(xf, w, labels, vocab_start, vocab, ignore_index, True)
+            target, top, total, loss_total = fwd(xf, w, labels, vocab_start, vocab, ignore_index, True)
             m = top.clone()
             dist.all_reduce(m, op=dist.ReduceOp.MAX, group=group)
             # the label's logit relative to the maximum comes from the one rank that holds its row
             local = labels - vocab_start
             counts = (labels >= 0) & (labels < vocab) & (labels != ignore_index)
             own = counts & (local >= 0) & (local < w.shape[0])
-            st = torch.stack([total * torch.exp(top - m), torch.where(own, target - m, torch.zeros_like(m))])
+            scale = torch.exp(top - m)
+            st = torch.stack([total * scale, loss_total * scale, torch.where(own, target - m, torch.zeros_like(m))])
             dist.all_reduce(st, group=group)
             total = st[0]
-            loss = torch.where(counts, torch.log(total) - st[1], torch.zeros_like(m))
+            loss = torch.where(counts, torch.log(st[1]) - st[2], torch.zeros_like(m))
         ctx.save_for_backward(x, w, labels, m, total)
         ctx.rest = (vocab_start, vocab, ignore_index)
         ctx.mode, ctx.group = mode, group
@@ -730,6 +732,9 @@ def linear_cross_entropy(x, w, labels, vocab_start: int = 0, mode: Optional[str]
     accumulates in fp32 into ``main_grad`` where the weight has one.  With a tensor-parallel ``group`` the weight is this
     rank's rows ``[vocab_start, vocab_start + V)`` (equal shares) and ``mode`` is that of the output layer: ``"col"`` or,
     with x split along the sequence, ``"col_sp"`` (labels are then those of the whole sequence)."""
+    if group is None and vocab_start == 0 and use_native(x) and not hasattr(w, "main_grad"):
+        # (the extension checks the arguments)
+        return ext().linear_ce(x, w, labels.contiguous(), ignore_index, LINEAR_CE_PIECE)
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"x must be [T, H] and w [V, H], got {tuple(x.shape)} and {tuple(w.shape)}")
     if x.dtype != w.dtype:

@@ -222,13 +222,15 @@ def _ce_rows(labels, col0, vocab, ignore, V):
 
 def linear_ce_fwd(x, w, labels, col0, vocab, ignore, raw):
     """(loss, maximum, sum of exponentials) over this rank's columns; with ``raw`` the label's logit (0 where another
-    rank holds it) in place of the loss."""
+    rank holds it), maximum, sum, and the sum for the loss (the kernels exchange the label's own term there)."""
     z = x.float() @ w.float().t()
     m = z.max(-1).values
     s = torch.exp(z - m[:, None]).sum(-1)
     counts, own, col = _ce_rows(labels, col0, vocab, ignore, w.shape[0])
     t = torch.where(own, z.gather(1, col[:, None]).squeeze(1), torch.zeros_like(m))
-    return (t if raw else torch.where(counts, torch.log(s) + (m - t), torch.zeros_like(m))), m, s
+    if raw:
+        return t, m, s, s
+    return torch.where(counts, torch.log(s) + (m - t), torch.zeros_like(m)), m, s
 
 
 def linear_ce_bwd(dloss, x, w, labels, top, total, col0, vocab, ignore, want_dx, want_dw, dw_accum, piece):

@@ -149,7 +149,7 @@ def test_raw_statistics_join_like_ranks():
     dx, dw = ext().linear_ce_bwd(dloss, x, w, labels, top, total, 0, 2048, -100, True, True, None, 0)
     st = [ext().linear_ce_fwd(x, w[h * 1024:(h + 1) * 1024], labels, h * 1024, 2048, -100, True) for h in (0, 1)]
     m = torch.maximum(st[0][1], st[1][1])
-    joined = sum(s * torch.exp(t - m) for _, t, s in st)
+    joined = sum(s * torch.exp(t - m) for _, t, _, s in st)
     target = st[0][0] + st[1][0]
     ok = (labels >= 0) & (labels < 2048)
     torch.testing.assert_close(torch.where(ok, torch.log(joined) + m - target, 0.0), whole, atol=1e-5, rtol=1e-6)
