@@ -425,6 +425,21 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
         } else {
           __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.C) + ti.c_off + (size_t)row * p.ldc + col0;
+          if constexpr (EPI == kCeGrad) {
+            if (p.ce.low_row) {  // (rows of the buffer are 16-byte aligned; columns past N are its padding)
+              __nv_bfloat16* low = dst + (size_t)p.ce.low_row * p.ldc;
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const float z = __uint_as_float(r[8 * v + j]);
+                  f[j] = z - __bfloat162float(__float2bfloat16_rn(z));
+                }
+                reinterpret_cast<uint4*>(low)[v] = pack8(f);
+              }
+            }
+          }
           if (ncols == 32 && ((reinterpret_cast<uintptr_t>(dst) & 15) == 0)) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
@@ -1332,7 +1347,8 @@ void gemm_grouped_wgrad(at::Tensor dy, at::Tensor x, at::Tensor seg, at::Tensor 
 
 // Logits product of the linear cross entropy: x [T, H] @ w [V, H]^T with a cross-entropy epilogue.  `grad` false: row
 // statistics into ce.part / ce.target, nothing else is written.  `grad` true: the gradient of the logits in bf16 into
-// out [T, V] (row stride a multiple of 8).  Up to 128 rows run as 128-row tiles on single SMs: the product then reads w
+// out [T, V] (row stride a multiple of 256 covering whole tiles), with ce.low_row = T <= 64 in out [2 T, V] with the
+// rounding errors, rounded again, below.  Up to 128 rows run as 128-row tiles on single SMs: the product then reads w
 // at memory speed and a 256-row tile would do twice the tensor work for nothing.
 void linear_ce_gemm(const at::Tensor& x, const at::Tensor& w, const CeArgs& ce, bool grad, const at::Tensor& out) {
   using namespace gk;
@@ -1346,6 +1362,8 @@ void linear_ce_gemm(const at::Tensor& x, const at::Tensor& w, const CeArgs& ce, 
   p.raster = raster_band(K);
   p.ce = ce;
   if (grad) {
+    TORCH_CHECK(out.stride(0) % BN == 0 && out.stride(0) >= (N + BN - 1) / BN * BN && (ce.low_row == 0 || ce.low_row <= 64) &&
+                    out.size(0) >= M + ce.low_row, "linear cross entropy: gradient buffer");
     p.C = out.data_ptr();
     p.ldc = (int)out.stride(0);
   }

@@ -6,7 +6,9 @@
 // backward, per piece [v0, v1) of the vocabulary, with P = (softmax(z) - onehot) dloss of that piece only:
 //           product again with the gradient epilogue -> P (bf16);   dx += P w[v0:v1] (fp32);   dw[v0:v1] (+)= P^T x.
 //           6 T V H operations: 2 more than with kept logits.
-// P is rounded to bf16 because the tensor cores multiply bf16; everything summed over V or T is summed in fp32.
+// P is rounded to bf16 because the tensor cores multiply bf16; everything summed over V or T is summed in fp32.  With
+// many rows these roundings average out next to that of the result.  Up to 64 rows one entry, the label's, can be all
+// there is to an element of dw, so P is kept as two bf16 rows, P and its rounding error: 2 T <= 128 rows cost no more.
 #include "linear_ce.cuh"
 
 #include <c10/cuda/CUDAGuard.h>
@@ -187,19 +189,23 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
   if (piece <= 0) piece = kPieceBytes / (2 * T);
   piece = std::min(whole, std::max<int64_t>(256, piece / 256 * 256));
   const int64_t pieces = (V + piece - 1) / piece;
-  auto P = at::empty({T, piece}, x.options());
+  const int64_t rows = T <= 64 ? 2 * T : T;  // of P
+  auto P = at::empty({rows, piece}, x.options());
+  const bool wants_w = want_dw || dw_accum.has_value();
+  auto xs = rows > T && wants_w ? at::cat({xr, xr}) : xr;
   CeArgs ce = ce_args(labels, col0, vocab, ignore);
   ce.top = top.data_ptr<float>();
   ce.sum = sum.data_ptr<float>();
+  ce.low_row = rows > T ? (int)T : 0;
   ce.dloss = g.data_ptr<float>();
   // dx of few rows has few output tiles and a long sum: split the sum over the SMs (fp32 parts joined in order)
-  const int64_t tiles1 = ((T + 127) / 128) * ((H + 255) / 256);
-  const bool split = want_dx && tiles1 * 2 <= num_sms() && V > 512;
+  const int64_t tiles1 = ((rows + 127) / 128) * ((H + 255) / 256);
+  const bool split = want_dx && (rows > T || tiles1 * 2 <= num_sms());
   // shares of a piece of n columns: one output tile for every SM, at least 512 columns a share
   auto shares = [&](int64_t n) { return std::max<int64_t>(1, std::min<int64_t>(num_sms() / tiles1, n / 512)); };
   const int64_t n_parts = split ? (pieces - 1) * shares(piece) + shares(V - (pieces - 1) * piece) : 1;
   at::Tensor parts;
-  if (want_dx && (split || pieces > 1)) parts = at::empty({n_parts, T, H}, f32);
+  if (want_dx && (split || pieces > 1)) parts = at::empty({n_parts, rows, H}, f32);
   int64_t part = 0;
   for (int64_t i = 0; i < pieces; ++i) {
     const int64_t v0 = i * piece, n = std::min(piece, V - v0);
@@ -214,14 +220,14 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
         gemm_tc(Pi, wi, false, false, pieces > 1 ? parts[0] : dx, i > 0, kBands);
       }
     }
-    if (dw_accum.has_value()) gemm_tc(Pi, xr, true, false, dw_accum->narrow(0, v0, n), true, kBands);
-    else if (want_dw) gemm_tc(Pi, xr, true, false, dw.narrow(0, v0, n), false, kBands);
+    if (dw_accum.has_value()) gemm_tc(Pi, xs, true, false, dw_accum->narrow(0, v0, n), true, kBands);
+    else if (want_dw) gemm_tc(Pi, xs, true, false, dw.narrow(0, v0, n), false, kBands);
   }
   if (parts.defined()) {
     const int64_t vecs = T * H / 4;
     const int grid = (int)std::min<int64_t>((vecs + 255) / 256, (int64_t)num_sms() * 8);
     parts_sum_kernel<<<grid, 256, 0, cur_stream()>>>(
-        reinterpret_cast<const float4*>(parts.data_ptr()), (int)n_parts, vecs,
+        reinterpret_cast<const float4*>(parts.data_ptr()), (int)(n_parts * (rows / T)), vecs,
         reinterpret_cast<__nv_bfloat16*>(dx.data_ptr()));
     EMB_LAUNCH_CHECK();
     count_launch();

@@ -23,6 +23,7 @@ struct CeArgs {
   const float* top;       // gradient: [T] maximum and sum of exponentials of the whole vocabulary
   const float* sum;
   const float* dloss;     // gradient: [T]
+  int low_row;            // gradient: 0, or the row that keeps what rounding to bf16 took from row 0, and so on
 };
 
 struct CeRow {
