@@ -291,10 +291,12 @@ __global__ void __launch_bounds__(kHeadThreads) heads_kernel(HeadParams p) {
 
 // ------------------------------------------------------------------------------------------ streamed kernel
 // The same operator for dense tensors.  Memory bound, so the data must not wait for registers: every warp streams
-// tiles of at most 2 KB of consecutive heads through a ring of its own in shared memory (cp.async.bulk, an mbarrier a
+// tiles of 2 or 4 KB of consecutive heads through a ring of its own in shared memory (cp.async.bulk, an mbarrier a
 // stage), turns them in place and sends them out with a bulk store.  Values pass without an instruction.  No warp waits
 // for another; the loads of the next stages are in flight while a tile is worked on.
-constexpr int kTileBytes = 2048;
+// Of one tensor, or each of two (dy and x).  Tiles of 4 KB take the rotation of 8192 x 2 x 48 x 128 from 69.7 to 65.6 us
+// (a copy of it: 61.5); with two tensors they would leave one CTA an SM.
+constexpr int tile_bytes(bool two) { return two ? 2048 : 4096; }
 constexpr int kStreamWarps = 8;
 constexpr unsigned kWaitPolls = 1u << 24;  // seconds of polling before a wait gives up
 
@@ -317,7 +319,8 @@ struct StreamParams {
   const void* w[2];
   float* part;  // [blocks, 2, d]
   int* err;
-  FastDiv per_token, slots, rows;  // heads of a token, of a group; tokens that share a row of the tables
+  FastDiv per_token, slots, turned, rows;  // heads of a token, of a group, turned ones of a group; tokens of a table row
+  int whole;  // tiles are whole groups
   int d, r, nq, nk;
   unsigned heads, tile_heads, tiles;
   float eps, inv_d;
@@ -438,15 +441,17 @@ __device__ __forceinline__ void vectors_of(int pair, int d, int r, int& a, int& 
   }
 }
 
-// A lane works on 16 channels of a head in packed fp32.  Every warp takes consecutive tiles, so a lane meets the heads
-// of one token one after the other and loads the token's cosines and sines once; the norm weights sit in shared memory
+// A lane works on 16 channels of a head in packed fp32 and keeps the cosines and sines while it meets heads of one token
+// (for the norm's backward a warp takes consecutive tiles, so that this is often); the norm weights sit in shared memory
 // as fp32, [class][quarter][lane] so that a lane's four 16-byte reads are free of bank conflicts.  What keeps the
 // kernel from the memory's rate otherwise is the number of instructions: 4 heads of 128 channels have about 350 issue
 // slots forward and 500 backward at the rate of a plain copy.
 template <typename T, int LPH, int STAGES, bool INTER, bool NORM, bool BWD>
-__global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 3) heads_stream_kernel(StreamParams p) {
+__global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_stream_kernel(StreamParams p) {
   constexpr int HPW = 32 / LPH;
   constexpr int BUFS = NORM && BWD ? 2 : 1;  // dy (or x), and x
+  constexpr bool RUNS = NORM && BWD;
+  constexpr int kTileBytes = tile_bytes(NORM && BWD);
   extern __shared__ __align__(128) uint8_t s_ring[];
   __shared__ uint64_t s_bar[kStreamWarps][STAGES];
   __shared__ __align__(16) float s_w[NORM ? 2 : 1][4][LPH][4];
@@ -455,7 +460,9 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 3) heads_
   uint64_t* bar = s_bar[warp];
   const unsigned head_bytes = p.d * (unsigned)sizeof(T);
   const unsigned long long warps = (unsigned long long)gridDim.x * kStreamWarps, me = blockIdx.x * kStreamWarps + warp;
-  const unsigned first = (unsigned)(p.tiles * me / warps), last = (unsigned)(p.tiles * (me + 1) / warps);
+  // the norm's backward, which is short of issue slots, takes consecutive tiles; the others walk the tensor together
+  const unsigned first = (unsigned)(RUNS ? p.tiles * me / warps : me);
+  const unsigned last = RUNS ? (unsigned)(p.tiles * (me + 1) / warps) : p.tiles, step = RUNS ? 1u : (unsigned)warps;
   const char* src0 = reinterpret_cast<const char*>(BWD ? p.dy : p.x);
   const char* src1 = reinterpret_cast<const char*>(p.x);
 
@@ -486,7 +493,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 3) heads_
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < STAGES; ++i)
-      if (first + i < last) load(first + i, i);
+      if (first + (unsigned long long)i * step < last) load(first + i * step, i);
   }
   f2 gw[NORM && BWD ? 2 : 1][8];
   if constexpr (NORM) {
@@ -513,7 +520,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 3) heads_
   unsigned have = ~0u;  // table row in cs / sn
   f2 cs[4], sn[4];
   unsigned it = 0;
-  for (unsigned tile = first; tile < last; ++tile, ++it) {
+  for (unsigned tile = first; tile < last; tile += step, ++it) {
     const int st = it % STAGES;
     if (!bulk_wait(bar + st, (it / STAGES) & 1)) {
       // a copy that does not arrive: report it, and leave after a bounded wait for the copies in flight
@@ -523,12 +530,23 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 3) heads_
     }
     uint8_t* buf = ring + st * BUFS * kTileBytes;
     const unsigned h0 = tile * p.tile_heads, n = min(p.tile_heads, p.heads - h0);
+    const unsigned work = p.whole ? p.slots.div(n) * (unsigned)(p.nq + p.nk) : n;
 #pragma unroll 1
-    for (unsigned i0 = 0; i0 < n; i0 += HPW) {
-      // heads past the end and values are read like any other (whatever the stage holds) but neither counted nor written
-      const unsigned i = i0 + sub, h = h0 + i;
-      const unsigned slot = h - p.slots.div(h) * p.slots.d;
-      const bool live = i < n && slot < (unsigned)(p.nq + p.nk);
+    for (unsigned i0 = 0; i0 < work; i0 += HPW) {
+      // tiles of whole groups: the i-th query or key head.  Else the i-th head; values are then read and worked on like
+      // any other but neither counted nor written, as are the lanes past the end
+      unsigned i = i0 + sub, slot;
+      bool live = i < work;
+      if (!live) i = 0;
+      if (p.whole) {
+        const unsigned g = p.turned.div(i);
+        slot = i - g * p.turned.d;
+        i = g * p.slots.d + slot;
+      } else {
+        slot = h0 + i - p.slots.div(h0 + i) * p.slots.d;
+        live = live && slot < (unsigned)(p.nq + p.nk);
+      }
+      const unsigned h = h0 + i;
       const bool is_k = slot >= (unsigned)p.nq;
       T* va = reinterpret_cast<T*>(buf + i * head_bytes) + oa;
       T* vb = reinterpret_cast<T*>(buf + i * head_bytes) + ob;
@@ -638,9 +656,10 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 3) heads_
                    : "memory");
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       // the stage of the tile before this one is free once its store has read it
-      if (it > 0 && tile + STAGES - 1 < last) {
+      const unsigned next = tile + (STAGES - 1) * step;  // (tiles and warps are below 2^30)
+      if (it > 0 && next < last) {
         asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        load(tile + STAGES - 1, (it - 1) % STAGES);
+        load(next, (it - 1) % STAGES);
       }
     }
     __syncwarp();
@@ -811,8 +830,8 @@ int split_grid(HeadParams& p, bool vec, int waves) {
 
 template <typename T, int LPH, bool INTER, bool NORM, bool BWD>
 void launch_stream(const StreamParams& p, int grid) {
-  constexpr int kStages = NORM && BWD ? 3 : 4;
-  constexpr int kSmem = kStreamWarps * kStages * kTileBytes * (NORM && BWD ? 2 : 1);
+  constexpr int kStages = 3;
+  constexpr int kSmem = kStreamWarps * kStages * tile_bytes(NORM && BWD) * (NORM && BWD ? 2 : 1);
   auto kern = heads_stream_kernel<T, LPH, kStages, INTER, NORM, BWD>;
   static bool done[kMaxDevices] = {};  // the shared-memory limit belongs to the device's context
   int dev = 0;
@@ -851,7 +870,7 @@ bool streams(const HeadParams& p, bool vec, const at::Tensor& t, const at::Tenso
          p.tokens * p.G * p.S >= kStreamHeads;
 }
 
-StreamParams stream_params(const HeadParams& p, int esize) {
+StreamParams stream_params(const HeadParams& p, int esize, bool two) {
   StreamParams q{};
   q.x = p.x;
   q.dy = p.dy;
@@ -872,7 +891,19 @@ StreamParams stream_params(const HeadParams& p, int esize) {
   q.inv_d = 1.f / (float)p.d;
   q.heads = (unsigned)(p.tokens * p.G * p.S);
   const unsigned hpw = 32u / std::max(4, lanes_per_head(p.d, 8));
-  q.tile_heads = std::max(hpw, kTileBytes / (unsigned)(p.d * esize) / hpw * hpw);
+  // A tile: as many heads as fit, or whole groups where that takes fewer rounds a head (values then cost none)
+  const unsigned fit = tile_bytes(two) / (unsigned)(p.d * esize), turned = (unsigned)(p.n[0] + p.n[1]);
+  q.turned = fast_div(std::max(1u, turned));
+  q.tile_heads = std::max(hpw, fit / hpw * hpw);
+  double best = 0.95 / hpw;
+  for (unsigned g = 1; turned > 0 && g * p.S <= fit; ++g) {
+    const double rounds = (double)((g * turned + hpw - 1) / hpw) / (g * p.S);
+    if (rounds <= best) {
+      best = rounds;
+      q.whole = 1;
+      q.tile_heads = g * p.S;
+    }
+  }
   q.tiles = (q.heads + q.tile_heads - 1) / q.tile_heads;
   return q;
 }
@@ -924,8 +955,8 @@ at::Tensor heads_fwd(at::Tensor qkv, at::Tensor cosv, at::Tensor sinv, int64_t n
   p.eps = (float)eps;
   vec = vec && rows_aligned(x);
   if (streams(p, vec, x, at::Tensor())) {
-    const StreamParams q = stream_params(p, (int)x.element_size());
-    by_type(x.scalar_type(), [&](auto t) { pick_stream<decltype(t)>(q, stream_grid(q, 3), interleaved, norm, false); });
+    const StreamParams q = stream_params(p, (int)x.element_size(), false);
+    by_type(x.scalar_type(), [&](auto t) { pick_stream<decltype(t)>(q, stream_grid(q, 2), interleaved, norm, false); });
     EMB_LAUNCH_CHECK();
     count_launch();
     return out;
@@ -995,8 +1026,8 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
   vec = vec && rows_aligned(g);
   const bool stream = streams(p, vec, g, x);
   StreamParams q{};
-  if (stream) q = stream_params(p, (int)g.element_size());
-  const int grid = stream ? stream_grid(q, norm ? 2 : 3) : split_grid(p, vec, kHeadWaves);
+  if (stream) q = stream_params(p, (int)g.element_size(), norm);
+  const int grid = stream ? stream_grid(q, 2) : split_grid(p, vec, kHeadWaves);
   const int nb0 = stream ? grid : p.block0[1], nb1 = stream ? grid : p.block0[2] - p.block0[1];
   at::Tensor part;
   if (norm) {
