@@ -70,6 +70,13 @@ class ModelConfig:
     max_tensor_parallel_size: int = 8
     seq_length: int = 512
     rotary_base: float = 10000.0
+    # share of each head's channels that turn, pairs side by side (GPT-J) instead of in halves, and how frequencies are
+    # stretched to longer contexts (Megatron's --rotary-percent, --rotary-interleaved, --use-rope-scaling)
+    rotary_percent: float = 1.0
+    rotary_interleaved: bool = False
+    rope_scaling: Optional[RopeScaling] = None
+    # RMSNorm of every query and key head before the rotation (Megatron's --qk-layernorm)
+    qk_layernorm: bool = False
     norm_epsilon: float = 1e-5
     # "RMSNorm" (Llama) or "LayerNorm" (Megatron's default, with a bias per norm: the reference's demo model)
     normalization: str = "RMSNorm"
@@ -80,6 +87,13 @@ class ModelConfig:
     moe_router_topk: int = 2
     moe_aux_loss_coeff: float = 1e-2
     moe_ffn_hidden_size: Optional[int] = None
+    # router: softmax after top-k, or (pre_softmax) the softmax over all experts kept as it is, or sigmoid scores divided
+    # by their sum; experts limited to the best group_topk of num_groups groups; weights times topk_scaling_factor
+    moe_router_score_function: str = "softmax"
+    moe_router_pre_softmax: bool = False
+    moe_router_num_groups: Optional[int] = None
+    moe_router_group_topk: Optional[int] = None
+    moe_router_topk_scaling_factor: Optional[float] = None
     # numerics
     params_dtype: str = "bf16"  # "bf16" | "fp32"
 
@@ -94,10 +108,27 @@ class ModelConfig:
         assert self.num_attention_heads % self.num_query_groups == 0
         if self.normalization not in ("RMSNorm", "LayerNorm"):
             raise ValueError(f"normalization must be RMSNorm or LayerNorm, got {self.normalization!r}")
+        if not 0.0 < self.rotary_percent <= 1.0 or self.rotary_dim % 2:
+            raise ValueError(f"rotary_percent must be in (0, 1] and give an even number of channels, got "
+                             f"{self.rotary_percent} of {self.head_dim}")
+        if self.moe_router_score_function not in ("softmax", "sigmoid"):
+            raise ValueError(f"moe_router_score_function must be softmax or sigmoid, got "
+                             f"{self.moe_router_score_function!r}")
+        if (self.moe_router_num_groups is None) != (self.moe_router_group_topk is None):
+            raise ValueError("moe_router_num_groups and moe_router_group_topk go together")
+        if self.moe_router_num_groups is not None and self.is_moe:
+            n, m = self.moe_router_num_groups, self.moe_router_group_topk
+            if n < 1 or self.num_experts % n or not 1 <= m <= n or m * (self.num_experts // n) < self.moe_router_topk:
+                raise ValueError(f"{m} of {n} groups of {self.num_experts} experts cannot give {self.moe_router_topk}")
 
     @property
     def head_dim(self) -> int:
         return self.hidden_size // self.num_attention_heads
+
+    @property
+    def rotary_dim(self) -> int:
+        """Channels of a head that turn."""
+        return int(self.head_dim * self.rotary_percent)
 
     @property
     def heads_per_group(self) -> int:
@@ -126,7 +157,7 @@ class ModelConfig:
     def num_params(self) -> int:
         h, f, v = self.hidden_size, self.ffn_hidden_size, self.padded_vocab_size
         norm = 2 * h if self.normalization == "LayerNorm" else h  # weight (+ bias)
-        per_layer = self.qkv_rows * h + h * h + 2 * norm
+        per_layer = self.qkv_rows * h + h * h + 2 * norm + (2 * self.head_dim if self.qk_layernorm else 0)
         if self.is_moe:
             per_layer += self.num_experts * (3 * self.moe_ffn_hidden_size * h) + self.num_experts * h
         else:
@@ -164,6 +195,9 @@ class TrainConfig:
     # context parallelism: "all_gather" (K/V gathered over the CP group), "p2p" (K/V passed round a ring) or
     # "a2a" (Ulysses: all-to-all from a sequence split to a query-group split and back)
     cp_comm_type: str = "all_gather"
+    # output layer and cross entropy without the [tokens, vocabulary] logits: the backward computes them again, a piece of
+    # the vocabulary at a time
+    fuse_linear_cross_entropy: bool = False
 
     def __post_init__(self):
         # Megatron flags kept for familiarity; the training core implements one setting of each

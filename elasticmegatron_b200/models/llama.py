@@ -8,10 +8,10 @@ is what lets a reshard swap the arena underneath it.
 Parallel structure per layer (Megatron-style, behaviour inferred from the reference's launch flags,
 run_e2e_demo.sh:77-95 and run_moe.sh:38-68):
 
-* input RMSNorm -> column-parallel QKV (AG over SP) -> RoPE -> causal GQA attention (ring over CP) ->
+* input RMSNorm -> column-parallel QKV (AG over SP) -> RoPE (with the query / key norms) -> causal GQA attention (ring over CP) ->
   row-parallel proj (RS over SP) -> residual;
 * RMSNorm -> column-parallel fc1 ``[W_t; V_t]`` -> SwiGLU -> row-parallel fc2 -> residual; or for MoE:
-  router (softmax over the top-k logits, switch load-balancing aux loss) -> all-to-all dispatch over EP ->
+  router (``models/moe.py``, switch load-balancing aux loss) -> all-to-all dispatch over EP ->
   grouped expert SwiGLU MLPs -> all-to-all combine.
 """
 from __future__ import annotations
@@ -24,7 +24,6 @@ from torch import nn
 
 from ..config import ModelConfig
 from ..ops import functional as F_
-from ..ops import reference as ref
 from ..models.spec import LocalParam
 from .moe import MoELayer
 from ..parallel.context_parallel import CP_COMM_TYPES, cp_attention, cp_ring_attention, cp_ulysses_attention
@@ -34,11 +33,11 @@ class RotaryCache:
     def __init__(self):
         self._c: Dict[tuple, tuple] = {}
 
-    def get(self, positions: torch.Tensor, dim: int, base: float, device):
-        key = (positions.shape[0], int(positions[0]), int(positions[-1]), dim, base, str(device))
+    def get(self, positions: torch.Tensor, dim: int, base: float, device, scaling=None):
+        key = (positions.shape[0], int(positions[0]), int(positions[-1]), dim, base, str(device), scaling)
         v = self._c.get(key)
         if v is None:
-            cos, sin = ref.rope_cos_sin(positions.cpu(), dim, base)
+            cos, sin = F_.rope_tables(positions.cpu(), dim, base, scaling)
             v = (cos.to(device), sin.to(device))
             self._c[key] = v
         return v
@@ -59,7 +58,8 @@ def cp_positions(seq: int, cp: int, cp_rank: int) -> torch.Tensor:
 
 class GPTStage(nn.Module):
     def __init__(self, cfg: ModelConfig, pstate, params: List[LocalParam], views: Dict[str, torch.Tensor],
-                 micro_batch_size: int, cp_comm_type: str = "all_gather", recompute: bool = False):
+                 micro_batch_size: int, cp_comm_type: str = "all_gather", recompute: bool = False,
+                 fuse_linear_cross_entropy: bool = False):
         super().__init__()
         if cp_comm_type not in CP_COMM_TYPES:
             raise ValueError(f"cp_comm_type must be one of {CP_COMM_TYPES}, got {cp_comm_type!r}")
@@ -74,6 +74,7 @@ class GPTStage(nn.Module):
         # full --recompute-method uniform --recompute-num-layers 1, which the reference's MoE launcher uses,
         # run_moe.sh:101-105): only each layer's input is kept; backward replays the layer's forward
         self.recompute = recompute
+        self.fuse_linear_cross_entropy = fuse_linear_cross_entropy
         self.tp_group = pstate.group("tp") if self.tp > 1 else None
         self.cp_group = pstate.group("cp") if self.cp > 1 else None
         self.cp_attention = {"all_gather": cp_attention, "p2p": cp_ring_attention,
@@ -149,7 +150,7 @@ class GPTStage(nn.Module):
         else:
             x = inp
         positions = cp_positions(cfg.seq_length, self.cp, self.ps.cp_rank if self.cp > 1 else 0)
-        cos, sin = _ROPE.get(positions, cfg.head_dim, cfg.rotary_base, x.device)
+        cos, sin = _ROPE.get(positions, cfg.rotary_dim, cfg.rotary_base, x.device, cfg.rope_scaling)
         aux_total = None
         recompute = self.recompute and torch.is_grad_enabled()
         # the residual stream is carried as (x, pending): the last branch output is added by the norm that
@@ -175,8 +176,11 @@ class GPTStage(nn.Module):
         w_out = self.params_by_name.get("output_layer.weight")
         if w_out is None:
             w_out = self.params_by_name["embedding.word_embeddings.weight"]
-        logits = F_.linear(x, w_out, self._mode("col"), self.tp_group)
         lab = labels.t().contiguous().view(-1)
+        if self.fuse_linear_cross_entropy:
+            losses = F_.linear_cross_entropy(x, w_out, lab, self.vocab_start, self._mode("col"), self.tp_group)
+            return losses, aux_total
+        logits = F_.linear(x, w_out, self._mode("col"), self.tp_group)
         losses = F_.vocab_parallel_cross_entropy(logits, lab, self.vocab_start, self.tp_group)
         return losses, aux_total
 
@@ -189,7 +193,12 @@ class GPTStage(nn.Module):
         x, h = self._add_norm(x, pending, f"decoder.layers.{i}.self_attention.linear_qkv.layer_norm_weight")
         qkv = F_.linear(h, self._p(i, "self_attention.linear_qkv.weight"), self._mode("col"), self.tp_group)
         qkv = qkv.view(seq_local, b, G_loc, hpg + 2, d)
-        qkv = F_.rope_qkv(qkv, cos, sin, hpg + 1)
+        if cfg.qk_layernorm:
+            qkv = F_.qk_norm_rope_qkv(qkv, self._p(i, "self_attention.q_layernorm.weight"),
+                                      self._p(i, "self_attention.k_layernorm.weight"), cos, sin, cfg.norm_epsilon,
+                                      cfg.rotary_interleaved)
+        else:
+            qkv = F_.rope_qkv(qkv, cos, sin, hpg + 1, cfg.rotary_interleaved)
         if self.cp > 1:
             attn = self.cp_attention(qkv, hpg, self.cp_group, self.ps.cp_rank, self.cp)
         else:

@@ -5,6 +5,10 @@ coefficient 1e-2, all-to-all dispatcher, grouped GEMM).  Routing: ``probs = soft
 aux loss ``= E * coeff / (T^2 * k) * sum_e(sum_t softmax(logits)[t, e] * count_e)`` (Switch Transformer
 load balancing).  Experts use ETP = 1: each EP rank holds ``E / EP`` whole experts stacked as
 ``fc1 [E_loc, 2f, h]`` / ``fc2 [E_loc, h, f]``.
+
+The other routers of :class:`~elasticmegatron_b200.config.ModelConfig` (softmax scores kept as they are, sigmoid scores,
+expert groups, scaled weights) and a selection bias (``MoELayer.expert_bias``) go through ``functional.moe_route``; the
+auxiliary loss is the same formula over that router's normalised scores.
 """
 from __future__ import annotations
 
@@ -190,15 +194,34 @@ class MoELayer:
         self.E = cfg.num_experts
         self.E_loc = self.E // self.ep
         self.k = cfg.moe_router_topk
+        # fp32 [E], added to the scores for the selection alone (balancing without an auxiliary loss).  It belongs to the
+        # training loop, which updates it from last_counts and sets it again on the layers that a reshard builds.
+        self.expert_bias = None
+        self.last_counts = None  # tokens of each expert in the last forward, of this rank
         s = pstate.strategy
         self.sp_group = pstate.group("tp") if (s.tensor_model_parallel_size > 1 and s.sequence_parallel) else None
 
     def __call__(self, h: torch.Tensor):
         f2 = self.w1.shape[1]
-        if (h.is_cuda and native_moe_enabled() and self.E <= 256 and self.k <= 8 and h.shape[1] % 64 == 0
-                and f2 % 64 == 0):
+        router_fits = self._general() or (self.E <= 256 and self.k <= 8)
+        if h.is_cuda and native_moe_enabled() and router_fits and h.shape[1] % 64 == 0 and f2 % 64 == 0:
             return self._native_forward(h)
         return self._torch_forward(h)
+
+    def _general(self) -> bool:
+        """Whether the router is another than softmax after top-k."""
+        c = self.cfg
+        return (self.expert_bias is not None or c.moe_router_score_function != "softmax" or c.moe_router_pre_softmax
+                or c.moe_router_num_groups is not None or c.moe_router_topk_scaling_factor is not None)
+
+    def _route(self, logits: torch.Tensor):
+        """(weights [T, k], experts [T, k], score_sum [E], counts [E]) of the general router."""
+        c = self.cfg
+        sigmoid = c.moe_router_score_function == "sigmoid"
+        factor = c.moe_router_topk_scaling_factor
+        return F_.moe_route(logits, self.k, c.moe_router_score_function, self.expert_bias, c.moe_router_num_groups or 1,
+                            c.moe_router_group_topk or 1, self.k > 1 if sigmoid else not c.moe_router_pre_softmax,
+                            1.0 if factor is None else factor)
 
     def _aux(self, score_sum: torch.Tensor, counts: torch.Tensor, T: int) -> torch.Tensor:
         E, k = self.E, self.k
@@ -219,8 +242,12 @@ class MoELayer:
         all-to-all)."""
         T = h.shape[0]
         E, k, E_loc, ep = self.E, self.k, self.E_loc, self.ep
-        logits = F_.linear(h, self.wr).float()
-        probs, score_sum, top, counts = _RouterFn.apply(logits, k)
+        logits = F_.linear(h, self.wr)
+        if self._general():
+            probs, top, score_sum, counts = self._route(logits)
+        else:
+            probs, score_sum, top, counts = _RouterFn.apply(logits.float(), k)
+        self.last_counts = counts
         aux = self._aux(score_sum, counts.to(torch.int64), T)
         gid = top.reshape(-1)
         if ep == 1:
@@ -264,10 +291,15 @@ class MoELayer:
         T = h.shape[0]
         E, k, E_loc, ep = self.E, self.k, self.E_loc, self.ep
         logits = F_.linear(h, self.wr).float()
-        top_logits, top_idx = logits.topk(k, dim=-1)
-        probs = torch.softmax(top_logits, -1)
-        scores = torch.softmax(logits, -1)
-        counts = torch.bincount(top_idx.reshape(-1), minlength=E)
+        if self._general():
+            probs, top_idx, score_sum, counts = self._route(logits)
+            top_idx, counts = top_idx.long(), counts.long()
+        else:
+            top_logits, top_idx = logits.topk(k, dim=-1)
+            probs = torch.softmax(top_logits, -1)
+            score_sum = torch.softmax(logits, -1).sum(0)
+            counts = torch.bincount(top_idx.reshape(-1), minlength=E)
+        self.last_counts = counts
         # Under sequence parallelism the aux loss is defined over the whole sequence: expert counts are
         # summed over the TP group and each rank contributes its tokens' share of sum_t softmax(logits).
         T_full, counts_full = T, counts
@@ -276,7 +308,7 @@ class MoELayer:
             dist.all_reduce(counts_full, group=self.sp_group)
             T_full = T * dist.get_world_size(self.sp_group)
         aux = (E * self.cfg.moe_aux_loss_coeff / (T_full * T_full * k)) * (
-            scores.sum(0) * counts_full.to(scores.dtype)).sum()
+            score_sum * counts_full.to(score_sum.dtype)).sum()
         flat = top_idx.reshape(-1)
         order = torch.argsort(flat, stable=True)
         token_of = order // k

@@ -42,6 +42,7 @@ class VParam:
     layer_id: Optional[int] = None
     expert_id: Optional[int] = None
     sp_partial: bool = False  # grad is a partial sum across TP ranks under sequence parallelism
+    tp_partial: bool = False  # grad is a partial sum across TP ranks always (each sees its own heads)
     weight_decay: bool = True
     init: str = "normal"  # "normal" | "ones" | "zeros"
     # name of the model parameter (within a layer / stage) this virtual param lives in
@@ -76,6 +77,8 @@ def _layer_params(cfg: ModelConfig) -> List[dict]:
              init="ones"),
         *_norm_bias(cfg, "self_attention.linear_qkv.layer_norm_weight"),
         dict(key="self_attention.linear_qkv.weight", shape=(cfg.qkv_rows, h), tp_dim=0),
+        *([dict(key=f"self_attention.{n}_layernorm.weight", shape=(cfg.head_dim,), tp_partial=True, weight_decay=False,
+                init="ones") for n in ("q", "k")] if cfg.qk_layernorm else []),
         dict(key="self_attention.linear_proj.weight", shape=(h, cfg.num_attention_heads * cfg.head_dim), tp_dim=1),
     ]
     if cfg.is_moe:
@@ -141,6 +144,7 @@ class LocalParam:
     # before the DP reduction; ``replica`` marks the last stage's copy, which the gradient norm skips
     tied: bool = False
     replica: bool = False
+    tp_partial: bool = False
 
     @property
     def numel(self) -> int:
@@ -223,7 +227,7 @@ def local_params(cfg: ModelConfig, vps: List[VParam], strategy, rank: int) -> Li
             name = vp.name
         out.append(LocalParam(name=name, key=vp.local_key, shape=shp, is_expert=False, layer_local=ll,
                               weight_decay=vp.weight_decay, sp_partial=vp.sp_partial, members=[(vp, 0)],
-                              tied=vp.tied_head))
+                              tied=vp.tied_head, tp_partial=vp.tp_partial))
     if head_copy is not None:
         out.append(head_copy)
     return out

@@ -189,16 +189,21 @@ class DistributedDataParallel:
             bl = self.layout.dense if kind == "dense" else self.layout.expert
             names = [bl.params[j].name for j in bl.bucket_params[b]]
             ps = [self.params[n] for n in names]
-            # SP-partial params need a TP all-reduce first, and tied-embedding copies a sum over the embedding
+            # TP-partial params (SP, head norms) need a TP all-reduce first, and tied-embedding copies a sum over the embedding
             # group (and, at PP=1, report ready from both the embedding and the head): keep their buckets for
             # the end of backward
-            if self.sp and any(p._local_param.sp_partial for p in ps):
+            if any(self._tp_partial(p) for p in ps):
                 continue
             if any(p._local_param.tied for p in ps):
                 continue
             for p in ps:
                 self._bucket_of[id(p)] = i
             self._bucket_sizes[i] = len(ps)
+
+    def _tp_partial(self, p) -> bool:
+        """The gradient is a partial sum over the TP ranks: each saw its part of the sequence, or its heads."""
+        lp = p._local_param
+        return (self.sp and lp.sp_partial) or (lp.tp_partial and self.ps.size("tp") > 1)
 
     def _launch_bucket(self, i: int):
         kind, b, s, e, zi, g, ig = self._bucket_views()[i]
@@ -219,8 +224,8 @@ class DistributedDataParallel:
         self.prepare()
 
     def finish_grad_sync(self) -> None:
-        if self.sp and self.ps.size("tp") > 1:
-            parts = [p.main_grad.view(-1) for p in self.params.values() if p._local_param.sp_partial]
+        if self.ps.size("tp") > 1:
+            parts = [p.main_grad.view(-1) for p in self.params.values() if self._tp_partial(p)]
             if parts:
                 flat = torch.cat(parts)
                 dist.all_reduce(flat, group=self.ps.group("tp"))

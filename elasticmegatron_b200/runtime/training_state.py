@@ -91,7 +91,7 @@ class TrainingState:
             self._alloc_opt()
         views = self._param_views() if not is_meta_device else self._meta_views()
         self.stage = GPTStage(self.cfg, self.ps, self.layout.params, views, tc.micro_batch_size, tc.cp_comm_type,
-                              tc.recompute)
+                              tc.recompute, tc.fuse_linear_cross_entropy)
         self.stage._training_state = self
         self.model = [self.stage]
         self.ddp = DistributedDataParallel(self.layout, self.ps, self.stage.params_by_name, self.param_flat,
@@ -174,7 +174,7 @@ class TrainingState:
             self.ddp.remove_hooks()
             self.stage = GPTStage(self.cfg, self.ps, self.layout.params, self._param_views(),
                                   self.train_cfg.micro_batch_size, self.train_cfg.cp_comm_type,
-                                  self.train_cfg.recompute)
+                                  self.train_cfg.recompute, self.train_cfg.fuse_linear_cross_entropy)
             self.stage._training_state = self
             self.model = [self.stage]
             self.ddp = DistributedDataParallel(self.layout, self.ps, self.stage.params_by_name, self.param_flat,

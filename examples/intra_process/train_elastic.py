@@ -34,6 +34,16 @@ def parse_args(argv=None):
     ap.add_argument("--seq-length", type=int, default=None)
     ap.add_argument("--num-experts", type=int, default=None, help="override the preset's expert count (MoE)")
     ap.add_argument("--moe-ffn", type=int, default=None, help="override the experts' ffn size")
+    ap.add_argument("--qk-layernorm", action="store_true", help="RMSNorm of every query and key head before the rotation")
+    ap.add_argument("--rotary-percent", type=float, default=1.0, help="share of each head's channels that turn")
+    ap.add_argument("--rotary-interleaved", action="store_true", help="turn neighbouring channels instead of halves")
+    ap.add_argument("--rope-scaling", default=None, metavar="KIND:FACTOR:CONTEXT",
+                    help="stretch rotary frequencies, e.g. yarn:8:4096 (kinds: linear, llama3, yarn)")
+    ap.add_argument("--router-score-function", default="softmax", choices=["softmax", "sigmoid"])
+    ap.add_argument("--router-groups", default=None, metavar="GROUPS:KEPT", help="choose experts of the best groups only")
+    ap.add_argument("--router-scaling", type=float, default=None, help="factor of the routing weights")
+    ap.add_argument("--fuse-linear-cross-entropy", action="store_true",
+                    help="output layer and loss without the [tokens, vocabulary] logits")
     ap.add_argument("--strategies", default=None,
                     help="comma list of strategy specs, e.g. ws8,ws2-tp2,ws4,ws2 (default: the reference's demo "
                          "schedule scaled to the job size)")
@@ -86,7 +96,7 @@ def main(argv=None):
                             **({"device_id": torch.device("cuda", local)} if use_cuda else {}))
 
     from elasticmegatron_b200 import ElasticMegatronManager
-    from elasticmegatron_b200.config import Args, TrainConfig, get_args, preset, set_args
+    from elasticmegatron_b200.config import Args, RopeScaling, TrainConfig, get_args, preset, set_args
     from elasticmegatron_b200.parallel.process_groups import create_all_groups
     from elasticmegatron_b200.parallel.strategy import ParallelStrategy
     from elasticmegatron_b200.runtime.train import train_step
@@ -102,13 +112,21 @@ def main(argv=None):
         over["num_experts"] = a.num_experts
     if a.moe_ffn:
         over["moe_ffn_hidden_size"] = a.moe_ffn
+    over.update(qk_layernorm=a.qk_layernorm, rotary_percent=a.rotary_percent, rotary_interleaved=a.rotary_interleaved,
+                moe_router_score_function=a.router_score_function, moe_router_topk_scaling_factor=a.router_scaling)
+    if a.rope_scaling:
+        kind, factor, context = a.rope_scaling.split(":")
+        over["rope_scaling"] = RopeScaling(kind, float(factor), int(context))
+    if a.router_groups:
+        over["moe_router_num_groups"], over["moe_router_group_topk"] = map(int, a.router_groups.split(":"))
     over["params_dtype"] = "bf16" if use_cuda else "fp32"  # the CUDA kernels are bf16; CPU ranks run fp32
     cfg = preset(a.model, **over)
     set_args(Args(model=cfg, train=TrainConfig(micro_batch_size=a.micro_batch_size,
                                                global_batch_size=a.global_batch_size, lr=a.lr, min_lr=a.min_lr,
                                                lr_warmup_iters=a.lr_warmup_iters, train_iters=a.train_iters,
                                                overlap_grad_reduce=a.overlap_grad_reduce,
-                                               cp_comm_type=a.cp_comm_type, recompute=a.recompute)))
+                                               cp_comm_type=a.cp_comm_type, recompute=a.recompute,
+                                               fuse_linear_cross_entropy=a.fuse_linear_cross_entropy)))
     specs = a.strategies.split(",") if a.strategies else default_schedule(world)
     strategies = [ParallelStrategy.parse(s) for s in specs]
     uniq = list(dict.fromkeys(strategies))
