@@ -114,6 +114,11 @@ at::Tensor tma_rows(const at::Tensor& t) {
   return ok ? t : at::empty(t.sizes(), t.options()).copy_(t);
 }
 
+// t.narrow(dim, at, n), without the view where that is all of t
+at::Tensor share(const at::Tensor& t, int64_t dim, int64_t at, int64_t n) {
+  return n == t.size(dim) ? t : t.narrow(dim, at, n);
+}
+
 CeArgs ce_args(const at::Tensor& labels, int64_t col0, int64_t vocab, int64_t ignore) {
   CeArgs ce{};
   ce.labels = labels.data_ptr<int64_t>();
@@ -137,14 +142,13 @@ std::vector<at::Tensor> linear_ce_fwd(at::Tensor x, at::Tensor w, at::Tensor lab
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t T = x.size(0), V = w.size(0);
   TORCH_CHECK(V > 0 && col0 >= 0 && col0 + V <= vocab && (raw || V == vocab), "columns outside the vocabulary");
-  auto f32 = x.options().dtype(at::kFloat);
-  auto out = at::empty({raw ? 4 : 3, T}, f32);
+  auto out = new_empty({raw ? 4 : 3, T}, x, at::kFloat);
   if (T == 0) return out.unbind(0);
   const int64_t tiles = (V + 255) / 256;
-  auto part = at::empty({tiles, T, 2}, f32), target = at::empty({T}, f32);
+  auto part = new_empty({tiles * T * 2 + T}, x, at::kFloat);  // and the labels' logits
   CeArgs ce = ce_args(labels, col0, vocab, ignore);
   ce.part = reinterpret_cast<float2*>(part.data_ptr<float>());
-  ce.target = target.data_ptr<float>();
+  ce.target = part.data_ptr<float>() + tiles * T * 2;
   auto xr = tma_rows(x), wr = tma_rows(w);
   linear_ce_gemm(xr, wr, ce, false, at::Tensor());
   float* o = out.data_ptr<float>();
@@ -165,7 +169,6 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
   check_ce(x, w, labels);
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t T = x.size(0), V = w.size(0), H = x.size(1);
-  auto f32 = x.options().dtype(at::kFloat);
   for (const auto& t : {top, sum})
     TORCH_CHECK(t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == T && t.device() == x.device(),
                 "the statistics of the forward pass must be fp32 [T]");
@@ -177,9 +180,9 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
                     dw_accum->size(1) == H && dw_accum->stride(1) == 1 && dw_accum->device() == x.device(),
                 "the weight gradient accumulator must be fp32 [V, H]");
   } else if (want_dw) {
-    dw = at::empty({V, H}, x.options());
+    dw = new_empty({V, H}, x, at::kBFloat16);
   }
-  if (want_dx) dx = at::empty({T, H}, x.options());
+  if (want_dx) dx = new_empty({T, H}, x, at::kBFloat16);
   if (T == 0) {
     if (dw.defined()) dw.zero_();
     return {dx, dw};
@@ -190,7 +193,7 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
   piece = std::min(whole, std::max<int64_t>(256, piece / 256 * 256));
   const int64_t pieces = (V + piece - 1) / piece;
   const int64_t rows = T <= 64 ? 2 * T : T;  // of P
-  auto P = at::empty({rows, piece}, x.options());
+  auto P = new_empty({rows, piece}, x, at::kBFloat16);
   const bool wants_w = want_dw || dw_accum.has_value();
   auto xs = rows > T && wants_w ? at::cat({xr, xr}) : xr;
   CeArgs ce = ce_args(labels, col0, vocab, ignore);
@@ -205,23 +208,23 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
   auto shares = [&](int64_t n) { return std::max<int64_t>(1, std::min<int64_t>(num_sms() / tiles1, n / 512)); };
   const int64_t n_parts = split ? (pieces - 1) * shares(piece) + shares(V - (pieces - 1) * piece) : 1;
   at::Tensor parts;
-  if (want_dx && (split || pieces > 1)) parts = at::empty({n_parts, rows, H}, f32);
+  if (want_dx && (split || pieces > 1)) parts = new_empty({n_parts, rows, H}, x, at::kFloat);
   int64_t part = 0;
   for (int64_t i = 0; i < pieces; ++i) {
     const int64_t v0 = i * piece, n = std::min(piece, V - v0);
-    auto Pi = P.narrow(1, 0, n), wi = wr.narrow(0, v0, n);
+    const auto Pi = share(P, 1, 0, n), wi = share(wr, 0, v0, n);
     ce.col0 = col0 + v0;
     linear_ce_gemm(xr, wi, ce, true, Pi);
     if (want_dx) {
       if (split) {
-        gemm_split_k(Pi, wi, parts.narrow(0, part, shares(n)));
+        gemm_split_k(Pi, wi, share(parts, 0, part, shares(n)));
         part += shares(n);
       } else {
         gemm_tc(Pi, wi, false, false, pieces > 1 ? parts[0] : dx, i > 0, kBands);
       }
     }
-    if (dw_accum.has_value()) gemm_tc(Pi, xs, true, false, dw_accum->narrow(0, v0, n), true, kBands);
-    else if (want_dw) gemm_tc(Pi, xs, true, false, dw.narrow(0, v0, n), false, kBands);
+    if (dw_accum.has_value()) gemm_tc(Pi, xs, true, false, share(*dw_accum, 0, v0, n), true, kBands);
+    else if (want_dw) gemm_tc(Pi, xs, true, false, share(dw, 0, v0, n), false, kBands);
   }
   if (parts.defined()) {
     const int64_t vecs = T * H / 4;

@@ -9,6 +9,7 @@
 
 #include <c10/cuda/CUDAStream.h>
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 
 namespace emb {
 
@@ -47,6 +48,11 @@ inline int* device_err_flag(int slot) {
 }
 
 inline cudaStream_t cur_stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+
+// An uninitialised CUDA tensor, straight from the allocator (half the host time of going through the dispatcher).
+inline at::Tensor new_empty(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
 
 inline int num_sms() {
   static int n = 0;

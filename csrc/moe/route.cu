@@ -560,10 +560,10 @@ std::vector<at::Tensor> moe_route_fwd(at::Tensor logits, int64_t k, bool sigmoid
   const c10::cuda::CUDAGuard guard(logits.device());
   auto x = row_contiguous(logits);
   RouteParams p = route_params(x, k, sigmoid, groups, topg, renorm, scaling);
-  auto f32 = x.options().dtype(at::kFloat), i32 = x.options().dtype(at::kInt);
-  auto weights = at::empty({p.T, k}, f32), experts = at::empty({p.T, k}, i32);
-  if (p.T == 0) return {weights, experts, at::zeros({p.E}, f32), at::zeros({p.E}, i32)};
-  auto score_sum = at::empty({p.E}, f32), counts = at::empty({p.E}, i32);
+  auto weights = new_empty({p.T, k}, x, at::kFloat), experts = new_empty({p.T, k}, x, at::kInt);
+  if (p.T == 0)
+    return {weights, experts, at::zeros({p.E}, weights.options()), at::zeros({p.E}, experts.options())};
+  auto score_sum = new_empty({p.E}, x, at::kFloat), counts = new_empty({p.E}, x, at::kInt);
   const int epl = lane_share(p.E), width = p.E / p.groups / epl;
   p.gwidth = p.gbest <= 2 && (p.E / p.groups) % epl == 0 && (width & (width - 1)) == 0 ? width : 0;
   // (twice the resident CTAs would give a second, partial wave)
@@ -576,7 +576,7 @@ std::vector<at::Tensor> moe_route_fwd(at::Tensor logits, int64_t k, bool sigmoid
     p.part = score_sum.data_ptr<float>();
     p.cpart = counts.data_ptr<int>();
   } else {
-    part = at::empty({2, grid, p.E}, f32);
+    part = new_empty({2, grid, p.E}, x, at::kFloat);
     p.part = part.data_ptr<float>();
     p.cpart = reinterpret_cast<int*>(p.part + (long long)grid * p.E);
   }
@@ -610,7 +610,7 @@ at::Tensor moe_route_bwd(at::Tensor logits, at::Tensor experts, c10::optional<at
   const c10::cuda::CUDAGuard guard(logits.device());
   auto x = row_contiguous(logits);
   RouteParams p = route_params(x, k, sigmoid, 1, 1, renorm, scaling);
-  auto dl = at::empty({p.T, p.E}, x.options());
+  auto dl = new_empty({p.T, p.E}, x, x.scalar_type());
   if (p.T == 0) return dl;
   TORCH_CHECK(experts.scalar_type() == at::kInt && experts.is_contiguous() && experts.size(0) == p.T,
               "experts must be the int32 tensor of the forward pass");

@@ -1,6 +1,8 @@
 // Autograd nodes of the decoder-step operators for CUDA tensors whose parameters keep ordinary gradients.  A node in C++
-// runs its backward in the engine's thread without entering Python (a forward and backward of small heads: 91 -> 75 us
+// runs its backward in the engine's thread without entering Python (a forward and backward of small heads: 91 -> 70 us
 // of one pass); parameters with a main_grad take the Python nodes of ops/functional.py, which know its hooks.
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
 namespace emb {
@@ -23,90 +25,151 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
 
 namespace {
 
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 using OptTensor = c10::optional<at::Tensor>;
 
+bool tracks(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
+at::Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
 OptTensor given(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
-struct HeadsNode : torch::autograd::Function<HeadsNode> {
-  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& qkv, const OptTensor& wq, const OptTensor& wk,
-                            const at::Tensor& cosv, const at::Tensor& sinv, int64_t nq, int64_t nk, double eps,
-                            bool interleaved) {
-    auto out = heads_fwd(qkv, cosv, sinv, nq, nk, interleaved, wq, wk, eps);
-    const bool norm = wq.has_value();
-    ctx->save_for_backward({norm ? qkv : at::Tensor(), norm ? *wq : at::Tensor(), norm ? *wk : at::Tensor(), cosv, sinv});
-    ctx->saved_data["nq"] = nq;
-    ctx->saved_data["nk"] = nk;
-    ctx->saved_data["eps"] = eps;
-    ctx->saved_data["inter"] = interleaved;
+// A node whose inputs are `inputs`, in the order of the gradients that apply() returns.
+template <typename N, typename... T>
+std::shared_ptr<N> new_node(const T&... inputs) {
+  auto n = std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
+  n->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+  return n;
+}
+
+struct HeadsNode : torch::autograd::Node {
+  SavedVariable qkv, wq, wk, cosv, sinv;
+  int64_t nq = 0, nk = 0;
+  double eps = 0;
+  bool interleaved = false;
+
+  variable_list apply(variable_list&& dy) override {
+    variable_list out(3);
+    if (!dy[0].defined()) return out;
+    at::NoGradGuard no_grad;
+    auto self = getptr();
+    const auto q = wq.unpack(self), k = wk.unpack(self);
+    auto g = heads_bwd(dy[0], given(qkv.unpack(self)), cosv.unpack(self), sinv.unpack(self), nq, nk, interleaved, given(q),
+                       given(k), eps, c10::nullopt, c10::nullopt);
+    for (size_t i = 0; i < g.size(); ++i) out[i] = std::move(g[i]);
     return out;
   }
-  static variable_list backward(AutogradContext* ctx, variable_list dy) {
-    const auto v = ctx->get_saved_variables();
-    auto g = heads_bwd(dy[0], given(v[0]), v[3], v[4], ctx->saved_data["nq"].toInt(), ctx->saved_data["nk"].toInt(),
-                       ctx->saved_data["inter"].toBool(), given(v[1]), given(v[2]), ctx->saved_data["eps"].toDouble(),
-                       c10::nullopt, c10::nullopt);
-    variable_list out(9);
-    for (size_t i = 0; i < g.size(); ++i) out[i] = g[i];
-    return out;
+  void release_variables() override {
+    for (auto* v : {&qkv, &wq, &wk, &cosv, &sinv}) v->reset_data();
   }
+  std::string name() const override { return "HeadsBackward"; }
 };
 
-struct RouteNode : torch::autograd::Function<RouteNode> {
-  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const OptTensor& bias, int64_t k,
-                               bool sigmoid, int64_t groups, int64_t topg, bool renorm, double scaling) {
-    auto r = moe_route_fwd(logits, k, sigmoid, bias, groups, topg, renorm, scaling);
-    ctx->save_for_backward({logits, r[1]});
-    ctx->saved_data["sigmoid"] = sigmoid;
-    ctx->saved_data["renorm"] = renorm;
-    ctx->saved_data["scaling"] = scaling;
-    ctx->set_materialize_grads(false);
-    ctx->mark_non_differentiable({r[1], r[3]});
-    return r;
-  }
-  static variable_list backward(AutogradContext* ctx, variable_list d) {
-    const auto v = ctx->get_saved_variables();
-    variable_list out(8);
-    if (d[0].defined() || d[2].defined())
-      out[0] = moe_route_bwd(v[0], v[1], given(d[0]), given(d[2]), ctx->saved_data["sigmoid"].toBool(),
-                             ctx->saved_data["renorm"].toBool(), ctx->saved_data["scaling"].toDouble());
+struct RouteNode : torch::autograd::Node {
+  SavedVariable logits, experts;
+  bool sigmoid = false, renorm = false;
+  double scaling = 1;
+
+  variable_list apply(variable_list&& d) override {  // of weights and score_sum
+    variable_list out(1);
+    if (!d[0].defined() && !d[1].defined()) return out;
+    at::NoGradGuard no_grad;
+    auto self = getptr();
+    out[0] = moe_route_bwd(logits.unpack(self), experts.unpack(self), given(d[0]), given(d[1]), sigmoid, renorm, scaling);
     return out;
   }
+  void release_variables() override {
+    logits.reset_data();
+    experts.reset_data();
+  }
+  std::string name() const override { return "MoERouteBackward"; }
 };
 
-struct LinearCeNode : torch::autograd::Function<LinearCeNode> {
-  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& labels,
-                            int64_t ignore, int64_t piece) {
-    auto r = linear_ce_fwd(x, w, labels, 0, w.size(0), ignore, false);
-    ctx->save_for_backward({x, w, labels, r[1], r[2]});
-    ctx->saved_data["ignore"] = ignore;
-    ctx->saved_data["piece"] = piece;
-    return r[0];
+struct LinearCeNode : torch::autograd::Node {
+  SavedVariable x, w, labels, top, sum;
+  int64_t ignore = 0, piece = 0;
+
+  variable_list apply(variable_list&& d) override {
+    variable_list out(2);
+    if (!d[0].defined()) return out;
+    at::NoGradGuard no_grad;
+    auto self = getptr();
+    const auto wv = w.unpack(self);
+    auto g = linear_ce_bwd(d[0], x.unpack(self), wv, labels.unpack(self), top.unpack(self), sum.unpack(self), 0, wv.size(0),
+                           ignore, should_compute_output(0), should_compute_output(1), c10::nullopt, piece);
+    return {std::move(g[0]), std::move(g[1])};
   }
-  static variable_list backward(AutogradContext* ctx, variable_list d) {
-    const auto v = ctx->get_saved_variables();
-    auto g = linear_ce_bwd(d[0], v[0], v[1], v[2], v[3], v[4], 0, v[1].size(0), ctx->saved_data["ignore"].toInt(),
-                           ctx->needs_input_grad(0), ctx->needs_input_grad(1), c10::nullopt,
-                           ctx->saved_data["piece"].toInt());
-    return {g[0], g[1], at::Tensor(), at::Tensor(), at::Tensor()};
+  void release_variables() override {
+    for (auto* v : {&x, &w, &labels, &top, &sum}) v->reset_data();
   }
+  std::string name() const override { return "LinearCrossEntropyBackward"; }
 };
 
 }  // namespace
 
 at::Tensor heads(at::Tensor qkv, OptTensor wq, OptTensor wk, at::Tensor cosv, at::Tensor sinv, int64_t nq, int64_t nk,
                  double eps, bool interleaved) {
-  return HeadsNode::apply(qkv, wq, wk, cosv, sinv, nq, nk, eps, interleaved);
+  at::Tensor out;
+  {
+    at::NoGradGuard no_grad;
+    out = heads_fwd(qkv, cosv, sinv, nq, nk, interleaved, wq, wk, eps);
+  }
+  const auto q = or_none(wq), k = or_none(wk);
+  if (at::GradMode::is_enabled() && (tracks(qkv) || tracks(q) || tracks(k))) {
+    auto n = new_node<HeadsNode>(qkv, q, k);
+    if (q.defined()) {  // the rotation alone needs no input for its gradient
+      n->qkv = SavedVariable(qkv, false);
+      n->wq = SavedVariable(q, false);
+      n->wk = SavedVariable(k, false);
+    }
+    n->cosv = SavedVariable(cosv, false);
+    n->sinv = SavedVariable(sinv, false);
+    n->nq = nq;
+    n->nk = nk;
+    n->eps = eps;
+    n->interleaved = interleaved;
+    torch::autograd::set_history(out, n);
+  }
+  return out;
 }
 
 std::vector<at::Tensor> moe_route(at::Tensor logits, OptTensor bias, int64_t k, bool sigmoid, int64_t groups, int64_t topg,
                                   bool renorm, double scaling) {
-  return RouteNode::apply(logits, bias, k, sigmoid, groups, topg, renorm, scaling);
+  std::vector<at::Tensor> r;
+  {
+    at::NoGradGuard no_grad;
+    r = moe_route_fwd(logits, k, sigmoid, bias, groups, topg, renorm, scaling);
+  }
+  if (at::GradMode::is_enabled() && tracks(logits)) {
+    auto n = new_node<RouteNode>(logits);
+    n->logits = SavedVariable(logits, false);
+    n->experts = SavedVariable(r[1], false);
+    n->sigmoid = sigmoid;
+    n->renorm = renorm;
+    n->scaling = scaling;
+    torch::autograd::set_history(r[0], n);
+    torch::autograd::set_history(r[2], n);
+  }
+  return r;
 }
 
 at::Tensor linear_ce(at::Tensor x, at::Tensor w, at::Tensor labels, int64_t ignore, int64_t piece) {
-  return LinearCeNode::apply(x, w, labels, ignore, piece);
+  std::vector<at::Tensor> r;
+  {
+    at::NoGradGuard no_grad;
+    r = linear_ce_fwd(x, w, labels, 0, w.dim() == 2 ? w.size(0) : 0, ignore, false);
+  }
+  if (at::GradMode::is_enabled() && (tracks(x) || tracks(w))) {
+    auto n = new_node<LinearCeNode>(x, w);
+    n->x = SavedVariable(x, false);
+    n->w = SavedVariable(w, false);
+    n->labels = SavedVariable(labels, false);
+    n->top = SavedVariable(r[1], false);
+    n->sum = SavedVariable(r[2], false);
+    n->ignore = ignore;
+    n->piece = piece;
+    torch::autograd::set_history(r[0], n);
+  }
+  return r[0];
 }
 
 }  // namespace emb

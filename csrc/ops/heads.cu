@@ -946,7 +946,7 @@ at::Tensor heads_fwd(at::Tensor qkv, at::Tensor cosv, at::Tensor sinv, int64_t n
     p.w[1] = wk->data_ptr();
     vec = vec && (uintptr_t)p.w[0] % 16 == 0 && (uintptr_t)p.w[1] % 16 == 0;
   }
-  auto out = at::empty(x.sizes(), x.options());
+  auto out = new_empty(x.sizes(), x, x.scalar_type());
   if (out.numel() == 0) return out;
   p.x = x.data_ptr();
   p.xs = x.stride(0);
@@ -994,7 +994,7 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
     p.xb = x.stride(1);
     vec = vec && rows_aligned(x) && (uintptr_t)p.w[0] % 16 == 0 && (uintptr_t)p.w[1] % 16 == 0;
   }
-  auto dx = at::empty(g.sizes(), g.options());
+  auto dx = new_empty(g.sizes(), g, g.scalar_type());
   std::vector<at::Tensor> res{dx};
   float* acc[2] = {nullptr, nullptr};
   void* dw[2] = {nullptr, nullptr};
@@ -1007,7 +1007,7 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
         acc[i] = (*a)->data_ptr<float>();
         res.emplace_back();
       } else {
-        res.push_back(at::empty({p.d}, g.options()));
+        res.push_back(new_empty({p.d}, g, g.scalar_type()));
         dw[i] = res.back().data_ptr();
       }
       ++i;
@@ -1031,7 +1031,7 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
   const int nb0 = stream ? grid : p.block0[1], nb1 = stream ? grid : p.block0[2] - p.block0[1];
   at::Tensor part;
   if (norm) {
-    part = at::empty({nb0 + nb1, p.d}, g.options().dtype(at::kFloat));
+    part = new_empty({nb0 + nb1, p.d}, g, at::kFloat);
     p.part = q.part = part.data_ptr<float>();
   }
   by_type(g.scalar_type(), [&](auto t) {
