@@ -155,6 +155,8 @@ struct Params {
   int a_mn, b_mn;  // operand majorness
   int* err;
   int split_tail;  // 2-SM kernel: run the last partial wave as 256 x 128 half tiles when they fit in one wave
+  int splits;      // 2-SM kernel: > 1 cuts K into that many equal shares, share i into rows [i * split_rows, ...) of C
+  int split_rows;  // (through the tensor map tmC; split_rows is a multiple of 256)
   int raster;      // 2-SM kernel: width of the bands in which tiles are walked (0: no bands)
   int m_fast;      // measurement only (EMB_GEMM_RASTER=m): m blocks vary fastest whatever the shape
   int no_store;    // 2-SM kernel, measurement only: read the accumulators but write no output
@@ -291,6 +293,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                  "r"(TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  grid_dependency();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -633,12 +636,18 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
   // as many 256 x 128 halves in one wave, they do - the last wave then takes half as long (4096 x 4096
   // outputs: 256 tiles on 74 clusters = 3 full waves + 34 tiles -> 3.5 wave-times instead of 4).  Work unit u
   // maps to tile unit_tile(u); unit_half(u) is -1 for a whole tile, else which 128-column half.
+  const int splits = !AG && p.splits > 1 ? p.splits : 1;
   const int tail = AG ? 0 : num_tiles % num_clusters;
   const bool split_tail = !AG && p.split_tail && tail > 0 && 2 * tail <= num_clusters;
   const int full_tiles = split_tail ? num_tiles - tail : num_tiles;
-  const int num_units = split_tail ? full_tiles + 2 * tail : num_tiles;
-  auto unit_tile = [&](int u) -> int { return u < full_tiles ? u : full_tiles + ((u - full_tiles) >> 1); };
-  auto unit_half = [&](int u) -> int { return u < full_tiles ? -1 : ((u - full_tiles) & 1); };
+  const int num_units = split_tail ? full_tiles + 2 * tail : num_tiles * splits;
+  auto unit_tile = [&](int u) -> int {
+    return splits > 1 ? u % num_tiles : u < full_tiles ? u : full_tiles + ((u - full_tiles) >> 1);
+  };
+  auto unit_half = [&](int u) -> int { return splits > 1 || u < full_tiles ? -1 : ((u - full_tiles) & 1); };
+  // the k-blocks of a unit: all, or its share of them
+  auto unit_k0 = [&](int u) -> int { return splits > 1 ? (int)((long long)nk * (u / num_tiles) / splits) : 0; };
+  auto unit_k1 = [&](int u) -> int { return splits > 1 ? (int)((long long)nk * (u / num_tiles + 1) / splits) : nk; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -659,6 +668,7 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
                  "r"(TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
+  grid_dependency();
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
@@ -686,7 +696,7 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
             if (!got) { ok = false; *abort_flag = 1; break; }
           }
         }
-        for (int kb = 0; kb < nk; ++kb, ++it) {
+        for (int kb = unit_k0(u), kb0 = kb, kb1 = unit_k1(u); kb < kb1; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           const unsigned long long t0 = timing ? clk() : 0;
@@ -749,7 +759,7 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
         if (timing) t_wt += clk() - ta;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * BN;
-        for (int kb = 0; kb < nk; ++kb, ++it) {
+        for (int kb = unit_k0(u), kb0 = kb, kb1 = unit_k1(u); kb < kb1; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           const unsigned long long t0 = timing ? clk() : 0;
@@ -762,7 +772,7 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
           if (!(p.probe & 1)) {
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k) {
-              mma_pair(d_tmem, a_s + (kstep(p.a_mn, k) >> 4), b_s + (kstep(p.b_mn, k) >> 4), idesc, (kb | k) != 0);
+              mma_pair(d_tmem, a_s + (kstep(p.a_mn, k) >> 4), b_s + (kstep(p.b_mn, k) >> 4), idesc, ((kb - kb0) | k) != 0);
             }
           }
           commit_pair(&empty[s]);
@@ -852,7 +862,7 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
         // (16-byte chunk j of row r at chunk j ^ (r & 7): conflict-free writes) and one lane hands the block to
         // the TMA unit: a tensor store, or an fp32 add-reduction into C for the accumulating weight gradient.
         // Out-of-range rows / columns are clipped by the tensor map.
-        const int row0 = tile_m(t) * BM + 128 * rank + quarter * 32;
+        const int row0 = tile_m(t) * BM + 128 * rank + quarter * 32 + (splits > 1 ? u / num_tiles * p.split_rows : 0);
         const int cols = p.out_fp32 ? 32 : 64;
         const int steps = (hf >= 0 ? BN / 2 : BN) / cols;
 #pragma unroll 1
@@ -1128,7 +1138,7 @@ namespace gk2 {
 // shared-memory limit on each device the first time it is used there.
 template <bool AG, int EPI = gk::kStore>
 static void launch(int bk, const CUtensorMap& tA, const CUtensorMap& tB, const CUtensorMap& tC, const gk::Params& p,
-                   int clusters) {
+                   int clusters, bool early = false) {
   static bool attr_set[2][kMaxDevices] = {};
   int dev = 0;
   EMB_CUDA_CHECK(cudaGetDevice(&dev));
@@ -1144,13 +1154,14 @@ static void launch(int bk, const CUtensorMap& tA, const CUtensorMap& tB, const C
   cfg.blockDim = dim3(AG ? NUM_THREADS_AG : NUM_THREADS, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = cur_stream();
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1] = early_launch();
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = early ? 2 : 1;
   EMB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tA, tB, tC, p));
 }
 }  // namespace gk2
@@ -1215,7 +1226,8 @@ at::Tensor gemm_tc(at::Tensor a, at::Tensor b, bool trans_a, bool trans_b, c10::
   CUtensorMap tB = b_mn ? make_map(b.data_ptr(), K, N, b.stride(0), 64, 64) : make_map(b.data_ptr(), N, K, b.stride(0), 64, BN);
   Params p{};
   p.m_fast = raster_m_fast();
-  if (variant == 16) {  // auto, with the tiles walked in bands
+  const bool early = variant == 16;
+  if (variant == 16) {  // auto, with the tiles walked in bands, started while the kernel before it ends
     p.raster = raster_band(K);
     variant = 0;
   }
@@ -1253,7 +1265,7 @@ at::Tensor gemm_tc(at::Tensor a, at::Tensor b, bool trans_a, bool trans_b, c10::
     CUtensorMap tC = tA2;
     if (p.no_store == 0 && make_c_map(C, p.out_fp32, M, N, tC)) p.c_tma = c_tma_enabled() ? 1 : 0;
     const int clusters = (int)std::min<int64_t>(tiles2, num_sms() / 2);
-    gk2::launch<false>(bk, tA2, tB2, tC, p, clusters);
+    gk2::launch<false>(bk, tA2, tB2, tC, p, clusters, early);
   } else {
     gemm1_smem_attr();
     const int tiles = (int)(((M + BM - 1) / BM) * ((N + BN - 1) / BN));
@@ -1374,31 +1386,34 @@ void linear_ce_gemm(const at::Tensor& x, const at::Tensor& w, const CeArgs& ce, 
     if (grad) p.c_tma = make_c_map(out, false, M, N, tC) ? 1 : 0;
     const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
     const int clusters = (int)std::min<int64_t>(tiles, num_sms() / 2);
-    if (grad) gk2::launch<false, kCeGrad>(128, tA, tB, tC, p, clusters);
-    else gk2::launch<false, kCeStats>(128, tA, tB, tC, p, clusters);
+    if (grad) gk2::launch<false, kCeGrad>(128, tA, tB, tC, p, clusters, true);
+    else gk2::launch<false, kCeStats>(128, tA, tB, tC, p, clusters, true);
   } else {
     CUtensorMap tA = make_map(x.data_ptr(), M, K, x.stride(0), 64, BM), tB = make_map(w.data_ptr(), N, K, w.stride(0), 64, BN);
     const int grid = (int)std::min<int64_t>((N + BN - 1) / BN, num_sms());
     if (grad) {
       gemm1_smem_attr<kCeGrad>();
-      gemm_kernel<kCeGrad><<<grid, NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
+      launch_early(gemm_kernel<kCeGrad>, grid, NUM_THREADS, SMEM_BYTES, tA, tB, p);
     } else {
       gemm1_smem_attr<kCeStats>();
-      gemm_kernel<kCeStats><<<grid, NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
+      launch_early(gemm_kernel<kCeStats>, grid, NUM_THREADS, SMEM_BYTES, tA, tB, p);
     }
   }
   EMB_LAUNCH_CHECK();
   count_launch();
 }
 
-// parts[g] = a[:, share g of K] @ b[share g of K, :] in fp32 for equal shares of the 64-deep k-blocks (each has at
-// least one): a [M, K], b [K, N] bf16, parts [shares, M, N].  For products with few output tiles and a long K.
+// parts[g] = a[:, share g of K] @ b[share g of K, :] in fp32 for equal shares of the k-blocks (each has at least one):
+// a [M, K], b [K, N] bf16, parts [shares, >= M, N].  For products with few output tiles and a long K.  More than 128 rows
+// take 256 x 256 tiles on CTA pairs; parts then needs whole tiles of rows (the rows past M are zero).
 void gemm_split_k(const at::Tensor& a, const at::Tensor& b, const at::Tensor& parts) {
   using namespace gk;
   TORCH_CHECK(ok_2d(a) && ok_2d(b) && parts.scalar_type() == at::kFloat && parts.is_contiguous(), "gemm_split_k: operands");
-  const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
-  TORCH_CHECK(parts.size(0) >= 1 && parts.size(0) <= (K + BK - 1) / BK, "gemm_split_k: more shares than k-blocks");
-  CUtensorMap tA = make_map(a.data_ptr(), M, K, a.stride(0), 64, BM), tB = make_map(b.data_ptr(), K, N, b.stride(0), 64, 64);
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(1), shares = parts.size(0);
+  const bool pair = M > BM;
+  const int bk = pair ? 128 : BK;
+  TORCH_CHECK(shares >= 1 && shares <= (K + bk - 1) / bk, "gemm_split_k: more shares than k-blocks");
+  TORCH_CHECK(parts.size(1) >= (pair ? (M + 255) / 256 * 256 : M) && parts.size(2) == N && N % 4 == 0, "gemm_split_k: parts");
   Params p{};
   p.C = parts.data_ptr();
   p.M = (int)M;
@@ -1408,12 +1423,25 @@ void gemm_split_k(const at::Tensor& a, const at::Tensor& b, const at::Tensor& pa
   p.out_fp32 = 1;
   p.b_mn = 1;
   p.err = err_flag();
-  p.group_mode = 3;
-  p.groups = (int)parts.size(0);
-  p.group_c_stride = (long long)M * N;
-  gemm1_smem_attr();
-  const int64_t tiles = p.groups * ((M + BM - 1) / BM) * ((N + BN - 1) / BN);
-  gemm_kernel<kStore><<<(int)std::min<int64_t>(tiles, num_sms()), NUM_THREADS, SMEM_BYTES, cur_stream()>>>(tA, tB, p);
+  if (pair) {
+    CUtensorMap tA = make_map(a.data_ptr(), M, K, a.stride(0), 64, 128), tB = make_map(b.data_ptr(), K, N, b.stride(0), 64, bk);
+    CUtensorMap tC;
+    const auto flat = parts.view({shares * parts.size(1), N});
+    TORCH_CHECK(make_c_map(flat, true, flat.size(0), N, tC), "gemm_split_k: parts must be 16-byte aligned");
+    p.c_tma = 1;
+    p.splits = (int)shares;
+    p.split_rows = (int)parts.size(1);
+    const int64_t tiles = shares * ((M + 255) / 256) * ((N + 255) / 256);
+    gk2::launch<false>(bk, tA, tB, tC, p, (int)std::min<int64_t>(tiles, num_sms() / 2), true);
+  } else {
+    CUtensorMap tA = make_map(a.data_ptr(), M, K, a.stride(0), 64, BM), tB = make_map(b.data_ptr(), K, N, b.stride(0), 64, 64);
+    p.group_mode = 3;
+    p.groups = (int)shares;
+    p.group_c_stride = (long long)parts.size(1) * N;
+    gemm1_smem_attr();
+    const int64_t tiles = shares * ((N + BN - 1) / BN);
+    launch_early(gemm_kernel<kStore>, (int)std::min<int64_t>(tiles, num_sms()), NUM_THREADS, SMEM_BYTES, tA, tB, p);
+  }
   EMB_LAUNCH_CHECK();
   count_launch();
 }

@@ -29,6 +29,7 @@ __global__ void __launch_bounds__(1024) ce_join_kernel(CeArgs ce, const __nv_bfl
                                                        float* __restrict__ out_top, float* __restrict__ out_sum,
                                                        float* __restrict__ out_loss_sum) {
   __shared__ float sm[32][33], ss[32][33];
+  grid_dependency();
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, row = blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f;
   if (row < T) {
@@ -77,13 +78,15 @@ __global__ void __launch_bounds__(1024) ce_join_kernel(CeArgs ce, const __nv_bfl
   out[t] = !own ? 0.f : raw ? dot : logf(z) + (top - dot);
 }
 
-// out[i] = bf16(sum over the n fp32 parts, in order)
-__global__ void parts_sum_kernel(const float4* __restrict__ parts, int n, int64_t vecs, __nv_bfloat16* __restrict__ out) {
+// out[i] = bf16(sum over the n fp32 parts, `stride` vectors apart, in order)
+__global__ void parts_sum_kernel(const float4* __restrict__ parts, int n, int64_t stride, int64_t vecs,
+                                 __nv_bfloat16* __restrict__ out) {
+  grid_dependency();
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < vecs; i += (int64_t)gridDim.x * blockDim.x) {
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int p = 0; p < n; ++p) {
-      const float4 v = parts[p * vecs + i];
+      const float4 v = parts[p * stride + i];
       a.x += v.x;
       a.y += v.y;
       a.z += v.z;
@@ -152,8 +155,8 @@ std::vector<at::Tensor> linear_ce_fwd(at::Tensor x, at::Tensor w, at::Tensor lab
   auto xr = tma_rows(x), wr = tma_rows(w);
   linear_ce_gemm(xr, wr, ce, false, at::Tensor());
   float* o = out.data_ptr<float>();
-  ce_join_kernel<<<(int)((T + 31) / 32), 1024, 0, cur_stream()>>>(
-      ce, reinterpret_cast<const __nv_bfloat16*>(xr.data_ptr()), xr.stride(0),
+  launch_early(
+      ce_join_kernel, (int)((T + 31) / 32), 1024, 0, ce, reinterpret_cast<const __nv_bfloat16*>(xr.data_ptr()), xr.stride(0),
       reinterpret_cast<const __nv_bfloat16*>(wr.data_ptr()), wr.stride(0), (int)x.size(1), (int)T, (int)tiles, (int)V, raw, o,
       o + T, o + 2 * T, raw ? o + 3 * T : nullptr);
   EMB_LAUNCH_CHECK();
@@ -201,14 +204,18 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
   ce.sum = sum.data_ptr<float>();
   ce.low_row = rows > T ? (int)T : 0;
   ce.dloss = g.data_ptr<float>();
-  // dx of few rows has few output tiles and a long sum: split the sum over the SMs (fp32 parts joined in order)
-  const int64_t tiles1 = ((rows + 127) / 128) * ((H + 255) / 256);
-  const bool split = want_dx && (rows > T || tiles1 * 2 <= num_sms());
-  // shares of a piece of n columns: one output tile for every SM, at least 512 columns a share
-  auto shares = [&](int64_t n) { return std::max<int64_t>(1, std::min<int64_t>(num_sms() / tiles1, n / 512)); };
+  // dx of few rows has few output tiles and a long sum: split the sum over the SMs (fp32 parts joined in order).  Up to 128
+  // rows of P a share is a 128 x 256 tile on an SM; above, 256 x 256 on a pair, in buffers of whole tiles of rows
+  // (512 x 129024 x 4096: 572 -> 436 us against whole sums on single SMs).
+  const bool pair = rows > 128;
+  const int64_t tiles = pair ? ((rows + 255) / 256) * ((H + 255) / 256) : (H + 255) / 256;
+  const int64_t slots = pair ? num_sms() / 2 : num_sms(), pad = pair ? (rows + 255) / 256 * 256 : rows;
+  const bool split = want_dx && (rows > T || (pair ? tiles : tiles * 2) <= slots);
+  // shares of a piece of n columns: one output tile for every SM or pair, at least 512 columns a share
+  auto shares = [&](int64_t n) { return std::max<int64_t>(1, std::min<int64_t>(slots / tiles, n / 512)); };
   const int64_t n_parts = split ? (pieces - 1) * shares(piece) + shares(V - (pieces - 1) * piece) : 1;
   at::Tensor parts;
-  if (want_dx && (split || pieces > 1)) parts = new_empty({n_parts, rows, H}, x, at::kFloat);
+  if (want_dx && (split || pieces > 1)) parts = new_empty({n_parts, split ? pad : T, H}, x, at::kFloat);
   int64_t part = 0;
   for (int64_t i = 0; i < pieces; ++i) {
     const int64_t v0 = i * piece, n = std::min(piece, V - v0);
@@ -227,11 +234,11 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
     else if (want_dw) gemm_tc(Pi, xs, true, false, share(dw, 0, v0, n), false, kBands);
   }
   if (parts.defined()) {
-    const int64_t vecs = T * H / 4;
+    // (with the low rows a part holds two summands of T rows each)
+    const int64_t vecs = T * H / 4, twice = rows / T;
     const int grid = (int)std::min<int64_t>((vecs + 255) / 256, (int64_t)num_sms() * 8);
-    parts_sum_kernel<<<grid, 256, 0, cur_stream()>>>(
-        reinterpret_cast<const float4*>(parts.data_ptr()), (int)(n_parts * (rows / T)), vecs,
-        reinterpret_cast<__nv_bfloat16*>(dx.data_ptr()));
+    launch_early(parts_sum_kernel, grid, 256, 0, reinterpret_cast<const float4*>(parts.data_ptr()), (int)(n_parts * twice),
+                 parts.size(1) / twice * H / 4, vecs, reinterpret_cast<__nv_bfloat16*>(dx.data_ptr()));
     EMB_LAUNCH_CHECK();
     count_launch();
   }

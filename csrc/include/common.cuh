@@ -54,6 +54,32 @@ inline at::Tensor new_empty(at::IntArrayRef sizes, const at::Tensor& like, at::S
   return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
 }
 
+// Programmatic dependent launch: a kernel launched "early" may start while the one before it on the stream still runs, up
+// to grid_dependency(), which waits for that one's end (and returns at once under an ordinary launch).  Chains of short
+// kernels so overlap one's launch and set-up with the other's last CTAs.
+inline cudaLaunchAttribute early_launch() {
+  cudaLaunchAttribute a = {};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
+template <typename... P, typename... A>
+void launch_early(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr = early_launch();
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = cur_stream();
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  EMB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, P(args)...));
+}
+__device__ __forceinline__ void grid_dependency() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 inline int num_sms() {
   static int n = 0;
   if (n == 0) {

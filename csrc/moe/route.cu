@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(1024) route_join_kernel(const float* __restric
                                                           int* __restrict__ counts) {
   __shared__ float sh[32][33];
   __shared__ int shc[32][33];
+  grid_dependency();
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
   float v = 0.f;
   int c = 0;
@@ -596,8 +597,8 @@ std::vector<at::Tensor> moe_route_fwd(at::Tensor logits, int64_t k, bool sigmoid
   });
   EMB_LAUNCH_CHECK();
   if (grid > 1)
-    route_join_kernel<<<(p.E + 31) / 32, 1024, 0, cur_stream()>>>(p.part, p.cpart, grid, p.E, score_sum.data_ptr<float>(),
-                                                                  counts.data_ptr<int>());
+    launch_early(route_join_kernel, (p.E + 31) / 32, 1024, 0, p.part, p.cpart, grid, p.E, score_sum.data_ptr<float>(),
+                 counts.data_ptr<int>());
   EMB_LAUNCH_CHECK();
   count_launch(grid > 1 ? 2 : 1);
   return {weights, experts, score_sum, counts};

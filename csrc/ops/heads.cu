@@ -698,6 +698,7 @@ template <typename T>
 __global__ void __launch_bounds__(1024) heads_join_kernel(const float* __restrict__ part, int d, int nb0, int nb1, int both,
                                                           T* dw0, T* dw1, float* acc0, float* acc1) {
   __shared__ float sh[32][33];
+  grid_dependency();
   // rows of `part`: those of class 0 and then those of class 1, or (`both`) the two of each block side by side
   const int cls = blockIdx.y, by = both ? 2 : 1;
   const int b0 = both ? 0 : cls ? nb0 : 0, b1 = both ? nb0 : cls ? nb0 + nb1 : nb0, shift = both ? cls : 0;
@@ -1039,8 +1040,8 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
     if (stream) pick_stream<T>(q, grid, interleaved, norm, true);
     else pick_shape<T>(p, grid, vec, interleaved, norm, true);
     if (norm) {
-      heads_join_kernel<T><<<dim3((p.d + 31) / 32, 2), 1024, 0, cur_stream()>>>(
-          p.part, p.d, nb0, nb1, stream, (T*)dw[0], (T*)dw[1], acc[0], acc[1]);
+      launch_early(heads_join_kernel<T>, dim3((p.d + 31) / 32, 2), 1024, 0, p.part, p.d, nb0, nb1, (int)stream, (T*)dw[0],
+                   (T*)dw[1], acc[0], acc[1]);
     }
   });
   EMB_LAUNCH_CHECK();
