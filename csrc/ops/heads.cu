@@ -133,7 +133,6 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 
 constexpr int kHeadThreads = 256;
-constexpr long long kStreamHeads = 8192;
 
 // One launch does all heads; the blocks are split between the classes (query, key, passing) in proportion to
 // their work, so that a block meets one weight vector and a lane always the same channels of it.
@@ -322,7 +321,7 @@ struct StreamParams {
   FastDiv per_token, slots, turned, rows;  // heads of a token, of a group, turned ones of a group; tokens of a table row
   int whole;  // tiles are whole groups
   int d, r, nq, nk;
-  unsigned heads, tile_heads, tiles;
+  unsigned heads, tile_heads, tiles, per_row;  // per_row: consecutive heads that share a row of the tables
   float eps, inv_d;
 };
 
@@ -517,7 +516,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
     __syncwarp();
   }
 
-  unsigned have = ~0u;  // table row in cs / sn
+  unsigned from = 0x80000000u;  // first head of the table row in cs / sn (none yet)
   f2 cs[4], sn[4];
   unsigned it = 0;
   for (unsigned tile = first; tile < last; tile += step, ++it) {
@@ -550,9 +549,9 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
       const bool is_k = slot >= (unsigned)p.nq;
       T* va = reinterpret_cast<T*>(buf + i * head_bytes) + oa;
       T* vb = reinterpret_cast<T*>(buf + i * head_bytes) + ob;
-      const unsigned row = p.rows.div(p.per_token.div(h));
-      if (live && row != have) {
-        have = row;
+      if (live && h - from >= p.per_row) {  // another row of the tables than the lane's last head had
+        const unsigned row = p.rows.div(p.per_token.div(h));
+        from = row * p.per_row;
         if constexpr (INTER) {
           if (ta) load4(p, row, oa / 2, cs, sn);
           if (tb) load4(p, row, ob / 2, cs + 2, sn + 2);
@@ -617,9 +616,10 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
           for (int j = 0; j < 8; ++j) a[j] = f2_mul(f2_mul(a[j], r2), w[j]);
           turn(a);
         } else {
+          // with b = g rstd:  dw += b x,  dx = b w - x rstd^2 mean(b w x)
           turn(a);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = f2_mul(x[j], r2);
+          for (int j = 0; j < 8; ++j) a[j] = f2_mul(a[j], r2);
           if (live) {
             if (is_k) {
 #pragma unroll
@@ -636,10 +636,10 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
             dot = f2_fma(a[j], x[j], dot);
           }
           const float2 d2 = f2_to(dot);
-          const float m = group_sum<LPH>(d2.x + d2.y) * -p.inv_d;
+          const float m = group_sum<LPH>(d2.x + d2.y) * (-p.inv_d * rstd * rstd);
           const f2 m2 = f2_of(m, m);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) a[j] = f2_mul(f2_fma(x[j], m2, a[j]), r2);
+          for (int j = 0; j < 8; ++j) a[j] = f2_fma(x[j], m2, a[j]);
         }
       } else {
         turn(a);
@@ -779,8 +779,18 @@ at::Tensor inner_contiguous(const at::Tensor& t) {
   return ok ? t : t.contiguous();
 }
 
-// Fills the parameters that forward and backward share; returns whether rows allow 8-channel vectors.
-bool set_up(HeadParams& p, const at::Tensor& t, const at::Tensor& cosv, const at::Tensor& sinv, int64_t nq, int64_t nk) {
+// Whether rows allow 8-channel vectors, in the direct and in the streamed kernel.
+struct Access {
+  bool direct, stream;
+  void need(bool ok) {
+    direct = direct && ok;
+    stream = stream && ok;
+  }
+};
+
+// Fills the parameters that forward and backward share.
+Access set_up(HeadParams& p, const at::Tensor& t, const at::Tensor& cosv, const at::Tensor& sinv, int64_t nq, int64_t nk,
+              bool interleaved) {
   TORCH_CHECK_VALUE(t.dim() == 5, "qkv must be [s, b, groups, slots, d]");
   const int64_t s = t.size(0), b = t.size(1), G = t.size(2), S = t.size(3), d = t.size(4);
   TORCH_CHECK_VALUE(nq >= 0 && nk >= 0 && nq + nk <= S, "more query and key heads than slots in a group");
@@ -804,7 +814,8 @@ bool set_up(HeadParams& p, const at::Tensor& t, const at::Tensor& cosv, const at
   p.n[0] = (int)nq;
   p.n[1] = (int)nk;
   p.n[2] = (int)(S - nq - nk);
-  return d % 8 == 0 && r % 16 == 0 && (uintptr_t)p.cosv % 16 == 0 && (uintptr_t)p.sinv % 16 == 0;
+  const bool ok = d % 8 == 0 && (uintptr_t)p.cosv % 16 == 0 && (uintptr_t)p.sinv % 16 == 0;
+  return {ok && r % 16 == 0, ok && r % (interleaved ? 8 : 16) == 0};
 }
 
 bool rows_aligned(const at::Tensor& t) {
@@ -865,10 +876,15 @@ void pick_stream(const StreamParams& p, int grid, bool inter, bool norm, bool bw
   }
 }
 
-// Dense tensors with 16-byte rows are streamed once there is more than a tile for every warp of the direct kernel.
-bool streams(const HeadParams& p, bool vec, const at::Tensor& t, const at::Tensor& other) {
-  return vec && t.is_contiguous() && (!other.defined() || other.is_contiguous()) &&
-         p.tokens * p.G * p.S >= kStreamHeads;
+// Dense tensors with 16-byte rows are streamed from a number of heads up, below which the rings' start costs more than the
+// loads that they hide.  Heads of 128, groups of 4 + 2, in L2, direct / streamed: forward 24576 heads 4.7 / 5.6 us, 49152
+// 7.4 / 7.3, 98304 11.8 / 11.2; backward with norm 12288 heads 9.0 / 8.6, 24576 13.2 / 11.5, 49152 19.2 / 14.4 (heads of 64
+// and single-head groups cross at 24576 to 49152 too).  They are streamed at any size where the interleaved turn
+// ends in the middle of the direct kernel's 16-channel pairs (r = 8 mod 16; the direct kernel would go by single channels).
+bool streams(const HeadParams& p, Access a, const at::Tensor& t, const at::Tensor& other) {
+  const long long heads = p.tokens * p.G * p.S, from = other.defined() ? 24576 : 49152;  // (other: the norm's backward)
+  return (a.direct ? heads >= from : a.stream) && t.is_contiguous() &&
+         (!other.defined() || other.is_contiguous());
 }
 
 StreamParams stream_params(const HeadParams& p, int esize, bool two) {
@@ -884,6 +900,7 @@ StreamParams stream_params(const HeadParams& p, int esize, bool two) {
   q.per_token = fast_div((unsigned)(p.G * p.S));
   q.slots = fast_div((unsigned)p.S);
   q.rows = fast_div(p.tb ? 1u : (unsigned)p.B);
+  q.per_row = (unsigned)(p.G * p.S) * q.rows.d;
   q.d = p.d;
   q.r = p.r;
   q.nq = p.n[0];
@@ -938,14 +955,14 @@ at::Tensor heads_fwd(at::Tensor qkv, at::Tensor cosv, at::Tensor sinv, int64_t n
   const c10::cuda::CUDAGuard guard(qkv.device());
   HeadParams p{};
   const bool norm = wq.has_value();
-  bool vec = set_up(p, qkv, cosv, sinv, nq, nk);
+  Access vec = set_up(p, qkv, cosv, sinv, nq, nk, interleaved);
   auto x = inner_contiguous(qkv);
   if (norm) {
     check_weights(wq, x, "q_weight");
     check_weights(wk, x, "k_weight");
     p.w[0] = wq->data_ptr();
     p.w[1] = wk->data_ptr();
-    vec = vec && (uintptr_t)p.w[0] % 16 == 0 && (uintptr_t)p.w[1] % 16 == 0;
+    vec.need((uintptr_t)p.w[0] % 16 == 0 && (uintptr_t)p.w[1] % 16 == 0);
   }
   auto out = new_empty(x.sizes(), x, x.scalar_type());
   if (out.numel() == 0) return out;
@@ -954,7 +971,7 @@ at::Tensor heads_fwd(at::Tensor qkv, at::Tensor cosv, at::Tensor sinv, int64_t n
   p.xb = x.stride(1);
   p.out = out.data_ptr();
   p.eps = (float)eps;
-  vec = vec && rows_aligned(x);
+  vec.need(rows_aligned(x));
   if (streams(p, vec, x, at::Tensor())) {
     const StreamParams q = stream_params(p, (int)x.element_size(), false);
     by_type(x.scalar_type(), [&](auto t) { pick_stream<decltype(t)>(q, stream_grid(q, 2), interleaved, norm, false); });
@@ -962,8 +979,8 @@ at::Tensor heads_fwd(at::Tensor qkv, at::Tensor cosv, at::Tensor sinv, int64_t n
     count_launch();
     return out;
   }
-  const int grid = split_grid(p, vec, kHeadWaves);
-  by_type(x.scalar_type(), [&](auto t) { pick_shape<decltype(t)>(p, grid, vec, interleaved, norm, false); });
+  const int grid = split_grid(p, vec.direct, kHeadWaves);
+  by_type(x.scalar_type(), [&](auto t) { pick_shape<decltype(t)>(p, grid, vec.direct, interleaved, norm, false); });
   EMB_LAUNCH_CHECK();
   count_launch();
   return out;
@@ -979,7 +996,7 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
   const c10::cuda::CUDAGuard guard(dy.device());
   HeadParams p{};
   const bool norm = wq.has_value();
-  bool vec = set_up(p, dy, cosv, sinv, nq, nk);
+  Access vec = set_up(p, dy, cosv, sinv, nq, nk, interleaved);
   auto g = inner_contiguous(dy);
   at::Tensor x;
   if (norm) {
@@ -993,7 +1010,7 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
     p.x = x.data_ptr();
     p.xs = x.stride(0);
     p.xb = x.stride(1);
-    vec = vec && rows_aligned(x) && (uintptr_t)p.w[0] % 16 == 0 && (uintptr_t)p.w[1] % 16 == 0;
+    vec.need(rows_aligned(x) && (uintptr_t)p.w[0] % 16 == 0 && (uintptr_t)p.w[1] % 16 == 0);
   }
   auto dx = new_empty(g.sizes(), g, g.scalar_type());
   std::vector<at::Tensor> res{dx};
@@ -1024,11 +1041,11 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
   p.db = g.stride(1);
   p.out = dx.data_ptr();
   p.eps = (float)eps;
-  vec = vec && rows_aligned(g);
+  vec.need(rows_aligned(g));
   const bool stream = streams(p, vec, g, x);
   StreamParams q{};
   if (stream) q = stream_params(p, (int)g.element_size(), norm);
-  const int grid = stream ? stream_grid(q, 2) : split_grid(p, vec, kHeadWaves);
+  const int grid = stream ? stream_grid(q, 2) : split_grid(p, vec.direct, kHeadWaves);
   const int nb0 = stream ? grid : p.block0[1], nb1 = stream ? grid : p.block0[2] - p.block0[1];
   at::Tensor part;
   if (norm) {
@@ -1038,7 +1055,7 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
   by_type(g.scalar_type(), [&](auto t) {
     using T = decltype(t);
     if (stream) pick_stream<T>(q, grid, interleaved, norm, true);
-    else pick_shape<T>(p, grid, vec, interleaved, norm, true);
+    else pick_shape<T>(p, grid, vec.direct, interleaved, norm, true);
     if (norm) {
       launch_early(heads_join_kernel<T>, dim3((p.d + 31) / 32, 2), 1024, 0, p.part, p.d, nb0, nb1, (int)stream, (T*)dw[0],
                    (T*)dw[1], acc[0], acc[1]);

@@ -48,6 +48,11 @@ HEADS = [  # s, b, G, hpg, d, r, per_seq
     (7, 1, 1, 2, 72, 32, False),    # an odd number of vectors
     (5, 1, 1, 1, 500, 250, False),
     (600, 1, 8, 1, 64, 16, False),
+    (1500, 2, 8, 4, 64, 64, False),  # from here on enough heads to be streamed
+    (2100, 1, 8, 1, 128, 32, False),
+    (901, 3, 6, 2, 80, 80, True),
+    (700, 1, 8, 8, 256, 256, False),
+    (13, 1, 2, 1, 96, 24, False),
     (3, 1, 1, 2, 64, 0, False),     # nothing turns
 ]
 
