@@ -258,3 +258,33 @@ def test_route_strided_rows_and_empty():
         F_.moe_route(torch.zeros(4, 8, device="cuda", dtype=torch.float64), 2)
     with pytest.raises(RuntimeError):
         F_.moe_route(torch.zeros(4, 8, device="cuda"), 2, bias=torch.zeros(8))
+
+
+# ------------------------------------------------------------------------------------------------ long tensors
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last tokens come out as in a call of their own."""
+    torch.cuda.empty_cache()
+    g = torch.Generator(device="cuda").manual_seed(9)
+    s, G, hpg, d = 700000, 4, 4, 128
+    x = torch.empty(s, 1, G, hpg + 2, d, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    assert x.numel() > 2 ** 31
+    ang = torch.rand(s, d // 2, generator=g, device="cuda") * 6.28
+    cos, sin = ang.cos(), ang.sin()
+    w = (1 + 0.2 * torch.randn(d, generator=g, device="cuda")).bfloat16()
+    y = F_.qk_norm_rope_qkv(x, w, w, cos, sin, 1e-5)
+    n = 70000
+    assert torch.equal(y[-n:], F_.qk_norm_rope_qkv(x[-n:], w, w, cos[-n:].clone(), sin[-n:].clone(), 1e-5))
+    del y
+    # strided rows (the direct kernel): every other token of twice as many
+    v = x[::2]
+    assert torch.equal(F_.rope_qkv(v, cos[::2].contiguous(), sin[::2].contiguous(), hpg + 1, interleaved=True)[-9:],
+                       F_.rope_qkv(v[-9:], cos[::2][-9:].contiguous(), sin[::2][-9:].contiguous(), hpg + 1,
+                                   interleaved=True))
+    del x, v
+    logits = torch.empty(4300000, 512, device="cuda").normal_(generator=g)
+    assert logits.numel() > 2 ** 31
+    a, b = F_.moe_route(logits, 4, "sigmoid", num_groups=8, group_topk=2), F_.moe_route(logits[-999:], 4, "sigmoid",
+                                                                                    num_groups=8, group_topk=2)
+    assert torch.equal(a[0][-999:], b[0]) and torch.equal(a[1][-999:], b[1]) and int(a[3].sum()) == 4 * 4300000
+    del logits, a, b
+    torch.cuda.empty_cache()

@@ -170,3 +170,45 @@ def test_refusals():
                 lambda: F_.linear_cross_entropy(x, w, labels.cpu()), lambda: F_.linear_cross_entropy(x, w.cpu(), labels)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_offsets_past_32_bits():
+    """A weight and a piece of P of more than 2^31 elements: the loss and gradients of labels at the end of the vocabulary."""
+    torch.cuda.empty_cache()
+    g = torch.Generator(device="cuda").manual_seed(11)
+    T, V, H = 9, 140000, 16384
+    w = torch.empty(V, H, device="cuda", dtype=torch.bfloat16).normal_(0, 0.02, generator=g)
+    assert w.numel() > 2 ** 31
+    x = torch.randn(T, H, generator=g, device="cuda").bfloat16()
+    labels = V - 1 - torch.arange(T, device="cuda")
+    z = torch.cat([x.double() @ w[v:v + 10000].double().t() for v in range(0, V, 10000)], 1)
+    want = torch.logsumexp(z, -1) - z.gather(1, labels[:, None]).squeeze(1)
+    w.requires_grad_()
+    loss = F_.linear_cross_entropy(x, w, labels)
+    p = torch.softmax(z, -1)
+    # the tensor cores cut their fp32 sum off at each of the H / 16 steps, by at most 2^-23 of a partial sum that grows to
+    # the logit: 2^-24 H / 16 of it in all.  The log of the sum moves by the softmax average of that.
+    bound = 3e-5 + 2.0 ** -24 * H / 16 * (p * z.abs()).sum(-1)
+    assert bool(((loss.double() - want).abs() <= bound).all())
+    gw, = torch.autograd.grad(loss.sum(), w)
+    p[torch.arange(T), labels] -= 1.0
+    for rows in (slice(0, 64), slice(V - 64, V)):
+        e = p[:, rows].t() @ x.double()
+        check(gw[rows], e, 1.1 * 2.0 ** -8 * (p[:, rows].t().abs() @ x.double().abs()))
+    del w, gw, z, p
+    # P of one piece: 20000 tokens by 110000 words
+    T, V, H = 20000, 110000, 64
+    x = torch.randn(T, H, generator=g, device="cuda").bfloat16().requires_grad_()
+    w = (torch.randn(V, H, generator=g, device="cuda") * 0.05).bfloat16()
+    labels = torch.randint(0, V, (T,), generator=g, device="cuda")
+    whole = {}
+    for piece in (V, 4096):
+        F_.LINEAR_CE_PIECE, keep = piece, F_.LINEAR_CE_PIECE
+        try:
+            loss = F_.linear_cross_entropy(x, w, labels)
+            whole[piece] = torch.autograd.grad(loss.sum(), x)[0].float()
+        finally:
+            F_.LINEAR_CE_PIECE = keep
+    # the same P and fp32 sums, in another order, rounded once
+    torch.testing.assert_close(whole[V], whole[4096], atol=1e-5, rtol=2.0 ** -7)
+    torch.cuda.empty_cache()
