@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, EPL <= 8 ? 2 : 1) route_fwd_
   int* s_cnt = reinterpret_cast<int*>(s_mem + 2 * kRouteWarps * ROW);
   float* s_grp = reinterpret_cast<float*>(s_cnt + p.E) + warp * p.groups * p.gstride;
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) s_cnt[e] = 0;
+  grid_dependency();
   __syncthreads();
   const bool by_group = p.groups > p.topg, by_logit = !p.bias && !by_group;
   const int per = p.E / p.groups;
@@ -391,6 +392,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_bwd_kernel(RouteParams
   __shared__ __align__(16) float s_ds[kRouteWarps][32 * EPL];  // ds of the chosen experts, 0 elsewhere
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float* row = s_ds[warp];
+  grid_dependency();
   float q[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
@@ -593,7 +595,7 @@ std::vector<at::Tensor> moe_route_fwd(at::Tensor logits, int64_t k, bool sigmoid
       if (!done[dev]) EMB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
       done[dev] = true;
     }
-    kern<<<grid, kRouteWarps * 32, smem, cur_stream()>>>(p);
+    launch_early(kern, grid, kRouteWarps * 32, smem, p);
   });
   EMB_LAUNCH_CHECK();
   if (grid > 1)
@@ -630,7 +632,7 @@ at::Tensor moe_route_bwd(at::Tensor logits, at::Tensor experts, c10::optional<at
   p.dlogits = dl.data_ptr();
   const int grid = std::min((p.T + kRouteWarps - 1) / kRouteWarps, num_sms() * 4);
   by_shape(x, [&](auto v, auto epl, auto vec) {
-    route_bwd_kernel<decltype(v), decltype(epl)::value, decltype(vec)::value><<<grid, kRouteWarps * 32, 0, cur_stream()>>>(p);
+    launch_early(route_bwd_kernel<decltype(v), decltype(epl)::value, decltype(vec)::value>, grid, kRouteWarps * 32, 0, p);
   });
   EMB_LAUNCH_CHECK();
   count_launch();

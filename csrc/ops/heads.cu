@@ -138,6 +138,7 @@ constexpr int kHeadThreads = 256;
 // their work, so that a block meets one weight vector and a lane always the same channels of it.
 template <typename T, int VEC, int LPH, int PPL, bool INTER, bool NORM, bool BWD>
 __global__ void __launch_bounds__(kHeadThreads) heads_kernel(HeadParams p) {
+  grid_dependency();
   const int cls = blockIdx.x >= p.block0[2] ? 2 : blockIdx.x >= p.block0[1] ? 1 : 0;
   const int blk = blockIdx.x - p.block0[cls];
   const int blocks = (cls == 2 ? gridDim.x : p.block0[cls + 1]) - p.block0[cls];
@@ -490,6 +491,9 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_at(bar + i)));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  grid_dependency();
+  if (lane == 0) {
 #pragma unroll
     for (int i = 0; i < STAGES; ++i)
       if (first + (unsigned long long)i * step < last) load(first + i * step, i);
@@ -723,7 +727,7 @@ __global__ void __launch_bounds__(1024) heads_join_kernel(const float* __restric
 template <typename T, int VEC, int LPH, int PPL, bool INTER, bool NORM, bool BWD>
 void launch_heads(const HeadParams& p, int grid) {
   const int smem = NORM && BWD ? (kHeadThreads / 32) * p.d * (int)sizeof(float) : 0;
-  heads_kernel<T, VEC, LPH, PPL, INTER, NORM, BWD><<<grid, kHeadThreads, smem, cur_stream()>>>(p);
+  launch_early(heads_kernel<T, VEC, LPH, PPL, INTER, NORM, BWD>, grid, kHeadThreads, smem, p);
 }
 
 template <typename T, int VEC, int LPH, int PPL>
@@ -852,7 +856,7 @@ void launch_stream(const StreamParams& p, int grid) {
     EMB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     done[dev] = true;
   }
-  kern<<<grid, kStreamWarps * 32, kSmem, cur_stream()>>>(p);
+  launch_early(kern, grid, kStreamWarps * 32, kSmem, p);
 }
 
 template <typename T, int LPH>
