@@ -358,29 +358,37 @@ __global__ void __launch_bounds__(kRouteWarps * 32, EPL <= 8 ? 2 : 1) route_fwd_
   }
 }
 
-// score_sum and counts from the CTAs' partials: 32 experts a CTA, 32 slices of the partials, joined by a fixed tree.
+// score_sum and counts from the CTAs' partials: 8 experts a CTA and 128 slices of the partials, so that a thread has two
+// or three loads to wait for at once; slices are joined by a fixed tree.
 __global__ void __launch_bounds__(1024) route_join_kernel(const float* __restrict__ part, const int* __restrict__ cpart,
                                                           int blocks, int E, float* __restrict__ score_sum,
                                                           int* __restrict__ counts) {
-  __shared__ float sh[32][33];
-  __shared__ int shc[32][33];
+  __shared__ float sh[32][9];
+  __shared__ int shc[32][9];
   grid_dependency();
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 8 + (lane & 7);
   float v = 0.f;
   int c = 0;
   if (e < E) {
-#pragma unroll 8
-    for (int b = slice; b < blocks; b += 32) {
+#pragma unroll 4
+    for (int b = threadIdx.x >> 3; b < blocks; b += 128) {
       v += part[(long long)b * E + e];
       c += cpart[(long long)b * E + e];
     }
   }
-  sh[slice][lane] = v;
-  shc[slice][lane] = c;
+  v += __shfl_xor_sync(kFull, v, 8);
+  c += __shfl_xor_sync(kFull, c, 8);
+  v += __shfl_xor_sync(kFull, v, 16);
+  c += __shfl_xor_sync(kFull, c, 16);
+  if (lane < 8) {
+    sh[warp][lane] = v;
+    shc[warp][lane] = c;
+  }
   __syncthreads();
-  v = warp_sum(sh[lane][slice]);
-  c = __reduce_add_sync(kFull, shc[lane][slice]);
-  const int o = blockIdx.x * 32 + slice;
+  if (warp >= 8) return;
+  v = warp_sum(sh[lane][warp]);
+  c = __reduce_add_sync(kFull, shc[lane][warp]);
+  const int o = blockIdx.x * 8 + warp;
   if (lane == 0 && o < E) {
     score_sum[o] = v;
     counts[o] = c;
@@ -599,7 +607,7 @@ std::vector<at::Tensor> moe_route_fwd(at::Tensor logits, int64_t k, bool sigmoid
   });
   EMB_LAUNCH_CHECK();
   if (grid > 1)
-    launch_early(route_join_kernel, (p.E + 31) / 32, 1024, 0, p.part, p.cpart, grid, p.E, score_sum.data_ptr<float>(),
+    launch_early(route_join_kernel, (p.E + 7) / 8, 1024, 0, p.part, p.cpart, grid, p.E, score_sum.data_ptr<float>(),
                  counts.data_ptr<int>());
   EMB_LAUNCH_CHECK();
   count_launch(grid > 1 ? 2 : 1);

@@ -709,24 +709,29 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
   }
 }
 
-// dw[cls][c] (+)= sum over the class's blocks of part[block][c]: 32 channels a CTA, 32 slices of the blocks, each
-// slice summed in order and the slices joined by a fixed tree.
+// dw[cls][c] (+)= sum over the class's blocks of part[block][c]: 8 channels a CTA and 128 slices of the blocks, so that a
+// thread has two or three loads to wait for at once; slices are joined by a fixed tree.
 template <typename T>
 __global__ void __launch_bounds__(1024) heads_join_kernel(const float* __restrict__ part, int d, int nb0, int nb1, int both,
                                                           T* dw0, T* dw1, float* acc0, float* acc1) {
-  __shared__ float sh[32][33];
+  __shared__ float sh[32][9];
   grid_dependency();
   // rows of `part`: those of class 0 and then those of class 1, or (`both`) the two of each block side by side
   const int cls = blockIdx.y, by = both ? 2 : 1;
   const int b0 = both ? 0 : cls ? nb0 : 0, b1 = both ? nb0 : cls ? nb0 + nb1 : nb0, shift = both ? cls : 0;
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 8 + (lane & 7);
   float v = 0.f;
-  if (c < d)
-    for (int b = b0 + slice; b < b1; b += 32) v += part[((long long)b * by + shift) * d + c];
-  sh[slice][lane] = v;
+  if (c < d) {
+#pragma unroll 4
+    for (int b = b0 + (threadIdx.x >> 3); b < b1; b += 128) v += part[((long long)b * by + shift) * d + c];
+  }
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  v += __shfl_xor_sync(0xffffffffu, v, 16);
+  if (lane < 8) sh[warp][lane] = v;
   __syncthreads();
-  v = warp_sum(sh[lane][slice]);  // slices of channel blockIdx.x * 32 + slice
-  const int ch = blockIdx.x * 32 + slice;
+  if (warp >= 8) return;
+  v = warp_sum(sh[lane][warp]);
+  const int ch = blockIdx.x * 8 + warp;
   if (lane == 0 && ch < d) {
     float* acc = cls ? acc1 : acc0;
     if (acc) {
@@ -1074,7 +1079,7 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
     if (stream) pick_stream<T>(q, grid, interleaved, norm, true);
     else pick_shape<T>(p, grid, vec.direct, interleaved, norm, true);
     if (norm) {
-      launch_early(heads_join_kernel<T>, dim3((p.d + 31) / 32, 2), 1024, 0, p.part, p.d, nb0, nb1, (int)stream, (T*)dw[0],
+      launch_early(heads_join_kernel<T>, dim3((p.d + 7) / 8, 2), 1024, 0, p.part, p.d, nb0, nb1, (int)stream, (T*)dw[0],
                    (T*)dw[1], acc[0], acc[1]);
     }
   });
