@@ -1361,7 +1361,8 @@ void gemm_grouped_wgrad(at::Tensor dy, at::Tensor x, at::Tensor seg, at::Tensor 
 // statistics into ce.part / ce.target, nothing else is written.  `grad` true: the gradient of the logits in bf16 into
 // out [T, V] (row stride a multiple of 256 covering whole tiles), with ce.low_row = T <= 64 in out [2 T, V] with the
 // rounding errors, rounded again, below.  Up to 128 rows run as 128-row tiles on single SMs: the product then reads w
-// at memory speed and a 256-row tile would do twice the tensor work for nothing.
+// at memory speed and a 256-row tile would do twice the tensor work for nothing (129024 x 4096 weights: 128 rows on single
+// SMs 205 us, 129 rows on pairs 237 us).
 void linear_ce_gemm(const at::Tensor& x, const at::Tensor& w, const CeArgs& ce, bool grad, const at::Tensor& out) {
   using namespace gk;
   TORCH_CHECK(ok_2d(x) && ok_2d(w), "linear cross entropy: x and w need 16-byte aligned rows");

