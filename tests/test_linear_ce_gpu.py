@@ -212,3 +212,40 @@ def test_offsets_past_32_bits():
     # the same P and fp32 sums, in another order, rounded once
     torch.testing.assert_close(whole[V], whole[4096], atol=1e-5, rtol=2.0 ** -7)
     torch.cuda.empty_cache()
+
+
+def test_captured_in_a_graph():
+    """A step of all operators in one CUDA graph gives what the calls give one by one."""
+    g = torch.Generator(device="cuda").manual_seed(13)
+    x, w, labels, dloss = make(300, 3001, 128, seed=13)
+    x.requires_grad_(), w.requires_grad_()
+    qkv = torch.randn(2000, 2, 4, 6, 64, generator=g, device="cuda").bfloat16().requires_grad_()
+    nw = torch.ones(64, device="cuda").bfloat16().requires_grad_()
+    ang = torch.rand(2000, 32, generator=g, device="cuda")
+    cos, sin = ang.cos(), ang.sin()
+    logits = torch.randn(3000, 64, generator=g, device="cuda").requires_grad_()
+
+    def step():
+        y = F_.qk_norm_rope_qkv(qkv, nw, nw, cos, sin, 1e-5)
+        z = F_.rope_qkv(y, cos, sin, 5, interleaved=True)
+        wt, ex, ss, ct = F_.moe_route(logits, 4, "sigmoid", num_groups=8, group_topk=2, renormalize=True)
+        loss = F_.linear_cross_entropy(x, w, labels)
+        grads = torch.autograd.grad([z, wt, ss, loss], [qkv, nw, logits, x, w],
+                                    [torch.ones_like(z), wt.detach(), ss.detach(), dloss])
+        return [z, wt, ex, ss, ct, loss, *grads]
+
+    want = [t.detach().clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        for t in got:
+            t.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
