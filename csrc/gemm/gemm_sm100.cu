@@ -1359,7 +1359,7 @@ void gemm_grouped_wgrad(at::Tensor dy, at::Tensor x, at::Tensor seg, at::Tensor 
 
 // Logits product of the linear cross entropy: x [T, H] @ w [V, H]^T with a cross-entropy epilogue.  `grad` false: row
 // statistics into ce.part / ce.target, nothing else is written.  `grad` true: the gradient of the logits in bf16 into
-// out [T, V] (row stride a multiple of 256 covering whole tiles), with ce.low_row = T <= 64 in out [2 T, V] with the
+// out [T, V] (row stride a multiple of 256 covering whole tiles), with ce.low_row = T <= 128 in out [2 T, V] with the
 // rounding errors, rounded again, below.  Up to 128 rows run as 128-row tiles on single SMs: the product then reads w
 // at memory speed and a 256-row tile would do twice the tensor work for nothing (129024 x 4096 weights: 128 rows on single
 // SMs 205 us, 129 rows on pairs 237 us).
@@ -1375,7 +1375,7 @@ void linear_ce_gemm(const at::Tensor& x, const at::Tensor& w, const CeArgs& ce, 
   p.raster = raster_band(K);
   p.ce = ce;
   if (grad) {
-    TORCH_CHECK(out.stride(0) % BN == 0 && out.stride(0) >= (N + BN - 1) / BN * BN && (ce.low_row == 0 || ce.low_row <= 64) &&
+    TORCH_CHECK(out.stride(0) % BN == 0 && out.stride(0) >= (N + BN - 1) / BN * BN && ce.low_row <= BM &&
                     out.size(0) >= M + ce.low_row, "linear cross entropy: gradient buffer");
     p.C = out.data_ptr();
     p.ldc = (int)out.stride(0);
@@ -1404,13 +1404,13 @@ void linear_ce_gemm(const at::Tensor& x, const at::Tensor& w, const CeArgs& ce, 
   count_launch();
 }
 
-// parts[g] = a[:, share g of K] @ b[share g of K, :] in fp32 for equal shares of the k-blocks (each has at least one):
-// a [M, K], b [K, N] bf16, parts [shares, >= M, N].  For products with few output tiles and a long K.  More than 128 rows
+// parts[g] = op(a)[:, share g of K] @ b[share g of K, :] in fp32 for equal shares of the k-blocks (each has at least one):
+// op(a) [M, K] (a itself, or a [K, M] transposed), b [K, N] bf16, parts [shares, >= M, N].  For products with few output tiles and a long K.  More than 128 rows
 // take 256 x 256 tiles on CTA pairs; parts then needs whole tiles of rows (the rows past M are zero).
-void gemm_split_k(const at::Tensor& a, const at::Tensor& b, const at::Tensor& parts) {
+void gemm_split_k(const at::Tensor& a, const at::Tensor& b, bool trans_a, const at::Tensor& parts) {
   using namespace gk;
   TORCH_CHECK(ok_2d(a) && ok_2d(b) && parts.scalar_type() == at::kFloat && parts.is_contiguous(), "gemm_split_k: operands");
-  const int64_t M = a.size(0), K = a.size(1), N = b.size(1), shares = parts.size(0);
+  const int64_t M = a.size(trans_a ? 1 : 0), K = a.size(trans_a ? 0 : 1), N = b.size(1), shares = parts.size(0);
   const bool pair = M > BM;
   const int bk = pair ? 128 : BK;
   TORCH_CHECK(shares >= 1 && shares <= (K + bk - 1) / bk, "gemm_split_k: more shares than k-blocks");
@@ -1422,10 +1422,12 @@ void gemm_split_k(const at::Tensor& a, const at::Tensor& b, const at::Tensor& pa
   p.K = (int)K;
   p.ldc = (int)N;
   p.out_fp32 = 1;
+  p.a_mn = trans_a;
   p.b_mn = 1;
   p.err = err_flag();
   if (pair) {
-    CUtensorMap tA = make_map(a.data_ptr(), M, K, a.stride(0), 64, 128), tB = make_map(b.data_ptr(), K, N, b.stride(0), 64, bk);
+    CUtensorMap tA = trans_a ? make_map(a.data_ptr(), K, M, a.stride(0), 64, bk) : make_map(a.data_ptr(), M, K, a.stride(0), 64, 128);
+    CUtensorMap tB = make_map(b.data_ptr(), K, N, b.stride(0), 64, bk);
     CUtensorMap tC;
     const auto flat = parts.view({shares * parts.size(1), N});
     TORCH_CHECK(make_c_map(flat, true, flat.size(0), N, tC), "gemm_split_k: parts must be 16-byte aligned");
@@ -1435,7 +1437,8 @@ void gemm_split_k(const at::Tensor& a, const at::Tensor& b, const at::Tensor& pa
     const int64_t tiles = shares * ((M + 255) / 256) * ((N + 255) / 256);
     gk2::launch<false>(bk, tA, tB, tC, p, (int)std::min<int64_t>(tiles, num_sms() / 2), true);
   } else {
-    CUtensorMap tA = make_map(a.data_ptr(), M, K, a.stride(0), 64, BM), tB = make_map(b.data_ptr(), K, N, b.stride(0), 64, 64);
+    CUtensorMap tA = trans_a ? make_map(a.data_ptr(), K, M, a.stride(0), 64, 64) : make_map(a.data_ptr(), M, K, a.stride(0), 64, BM);
+    CUtensorMap tB = make_map(b.data_ptr(), K, N, b.stride(0), 64, 64);
     p.group_mode = 3;
     p.groups = (int)shares;
     p.group_c_stride = (long long)parts.size(1) * N;

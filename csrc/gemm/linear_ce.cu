@@ -10,8 +10,9 @@
 // TFLOP/s (the library's sustained rate: 1358); 4096 x 32000 x 4096: 3.27 ms; 250 x 32001 x 512: 76 us.
 //
 // P is rounded to bf16 because the tensor cores multiply bf16; everything summed over V or T is summed in fp32.  With
-// many rows these roundings average out next to that of the result.  Up to 64 rows one entry, the label's, can be all
-// there is to an element of dw, so P is kept as two bf16 rows, P and its rounding error: 2 T <= 128 rows cost no more.
+// many rows these roundings average out next to that of the result.  With few, one entry, the label's, can be all there is
+// to an element of dw, so up to 128 rows P is kept as two bf16 rows, P and its rounding error (weights of 129024 x 4096,
+// backward with 65 / 128 rows: 790 / 842 us; with one row each 733 / 732).
 #include "linear_ce.cuh"
 
 #include <c10/cuda/CUDAGuard.h>
@@ -81,9 +82,11 @@ __global__ void __launch_bounds__(1024) ce_join_kernel(CeArgs ce, const __nv_bfl
   out[t] = !own ? 0.f : raw ? dot : logf(z) + (top - dot);
 }
 
-// out[i] = bf16(sum over the n fp32 parts, `stride` vectors apart, in order)
-__global__ void parts_sum_kernel(const float4* __restrict__ parts, int n, int64_t stride, int64_t vecs,
-                                 __nv_bfloat16* __restrict__ out) {
+// Sum over the n fp32 parts, `stride` vectors apart, in order; with `low` each part holds a second summand that many vectors
+// further on.  Rounded into the dense bf16 `out`, or added to `accum` with `width` vectors in a row and `ld` elements between
+// rows.
+__global__ void parts_sum_kernel(const float4* __restrict__ parts, int n, int64_t stride, int64_t low, int64_t vecs,
+                                 __nv_bfloat16* __restrict__ out, float* __restrict__ accum, int width, int64_t ld) {
   grid_dependency();
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < vecs; i += (int64_t)gridDim.x * blockDim.x) {
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -94,11 +97,53 @@ __global__ void parts_sum_kernel(const float4* __restrict__ parts, int n, int64_
       a.y += v.y;
       a.z += v.z;
       a.w += v.w;
+      if (low) {
+        const float4 u = parts[p * stride + low + i];
+        a.x += u.x;
+        a.y += u.y;
+        a.z += u.z;
+        a.w += u.w;
+      }
     }
-    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(a.x, a.y), __floats2bfloat162_rn(a.z, a.w)};
-    reinterpret_cast<uint2*>(out)[i] = *reinterpret_cast<uint2*>(h);
+    if (accum) {
+      float* dst = accum + i / width * ld + i % width * 4;
+      dst[0] += a.x;
+      dst[1] += a.y;
+      dst[2] += a.z;
+      dst[3] += a.w;
+    } else {
+      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(a.x, a.y), __floats2bfloat162_rn(a.z, a.w)};
+      reinterpret_cast<uint2*>(out)[i] = *reinterpret_cast<uint2*>(h);
+    }
   }
 }
+
+// Joins parts [n, >= rows, H] into `rows` rows of dst (dense bf16, or fp32 that is added to).
+void sum_parts(const at::Tensor& parts, int64_t n, bool low, int64_t rows, const at::Tensor& dst) {
+  const int64_t H = parts.size(2), vecs = rows * H / 4;
+  const int grid = (int)std::min<int64_t>((vecs + 255) / 256, (int64_t)num_sms() * 8);
+  const bool add = dst.scalar_type() == at::kFloat;
+  launch_early(parts_sum_kernel, grid, 256, 0, reinterpret_cast<const float4*>(parts.data_ptr()), (int)n,
+               parts.size(1) * H / 4, low ? vecs : 0, vecs,
+               add ? nullptr : reinterpret_cast<__nv_bfloat16*>(dst.data_ptr()), add ? dst.data_ptr<float>() : nullptr,
+               (int)(H / 4), dst.stride(0));
+  EMB_LAUNCH_CHECK();
+  count_launch();
+}
+
+// How a product of few output tiles cuts its K: `shares` so that every SM (up to 128 rows, a 128 x 256 tile each) or pair
+// (256 x 256 tiles) gets one tile of at least 512 of K; 1: not at all.  `pad`: rows of a part.
+struct Split {
+  bool pair;
+  int64_t tiles, slots, pad;
+  Split(int64_t rows, int64_t cols) {
+    pair = rows > 128;
+    tiles = (pair ? (rows + 255) / 256 : 1) * ((cols + 255) / 256);
+    slots = pair ? num_sms() / 2 : num_sms();
+    pad = pair ? (rows + 255) / 256 * 256 : rows;
+  }
+  int64_t shares(int64_t k) const { return std::max<int64_t>(1, std::min(slots / tiles, k / 512)); }
+};
 
 void check_ce(const at::Tensor& x, const at::Tensor& w, const at::Tensor& labels) {
   TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && x.size(1) % 8 == 0 && x.size(1) > 0 &&
@@ -199,7 +244,7 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
   if (piece <= 0) piece = kPieceBytes / (2 * T);
   piece = std::min(whole, std::max<int64_t>(256, piece / 256 * 256));
   const int64_t pieces = (V + piece - 1) / piece;
-  const int64_t rows = T <= 64 ? 2 * T : T;  // of P
+  const int64_t rows = T <= 128 ? 2 * T : T;  // of P
   auto P = new_empty({rows, piece}, x, at::kBFloat16);
   const bool wants_w = want_dw || dw_accum.has_value();
   auto xs = rows > T && wants_w ? at::cat({xr, xr}) : xr;
@@ -208,18 +253,14 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
   ce.sum = sum.data_ptr<float>();
   ce.low_row = rows > T ? (int)T : 0;
   ce.dloss = g.data_ptr<float>();
-  // dx of few rows has few output tiles and a long sum: split the sum over the SMs (fp32 parts joined in order).  Up to 128
-  // rows of P a share is a 128 x 256 tile on an SM; above, 256 x 256 on a pair, in buffers of whole tiles of rows
-  // (512 x 129024 x 4096: 572 -> 436 us against whole sums on single SMs).
-  const bool pair = rows > 128;
-  const int64_t tiles = pair ? ((rows + 255) / 256) * ((H + 255) / 256) : (H + 255) / 256;
-  const int64_t slots = pair ? num_sms() / 2 : num_sms(), pad = pair ? (rows + 255) / 256 * 256 : rows;
-  const bool split = want_dx && (rows > T || (pair ? tiles : tiles * 2) <= slots);
-  // shares of a piece of n columns: one output tile for every SM or pair, at least 512 columns a share
-  auto shares = [&](int64_t n) { return std::max<int64_t>(1, std::min<int64_t>(slots / tiles, n / 512)); };
-  const int64_t n_parts = split ? (pieces - 1) * shares(piece) + shares(V - (pieces - 1) * piece) : 1;
+  // dx of few rows and dw of few words have few output tiles and a long sum: it is split, fp32 parts joined in order
+  // (dx of 512 x 129024 x 4096: 572 -> 436 us, dw of 8192 x 1000 x 512: 82 -> 26 us against whole sums on single SMs)
+  const Split sx(rows, H), sw(std::min(piece, V), H);
+  const bool split = want_dx && (rows > T || (sx.pair ? sx.tiles : sx.tiles * 2) <= sx.slots);
+  const bool split_w = wants_w && pieces == 1 && sw.shares(xs.size(0)) > 1;
+  const int64_t n_parts = split ? (pieces - 1) * sx.shares(piece) + sx.shares(V - (pieces - 1) * piece) : 1;
   at::Tensor parts;
-  if (want_dx && (split || pieces > 1)) parts = new_empty({n_parts, split ? pad : T, H}, x, at::kFloat);
+  if (want_dx && (split || pieces > 1)) parts = new_empty({n_parts, split ? sx.pad : T, H}, x, at::kFloat);
   int64_t part = 0;
   for (int64_t i = 0; i < pieces; ++i) {
     const int64_t v0 = i * piece, n = std::min(piece, V - v0);
@@ -228,24 +269,23 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
     linear_ce_gemm(xr, wi, ce, true, Pi);
     if (want_dx) {
       if (split) {
-        gemm_split_k(Pi, wi, share(parts, 0, part, shares(n)));
-        part += shares(n);
+        gemm_split_k(Pi, wi, false, share(parts, 0, part, sx.shares(n)));
+        part += sx.shares(n);
       } else {
         gemm_tc(Pi, wi, false, false, pieces > 1 ? parts[0] : dx, i > 0, kBands);
       }
     }
-    if (dw_accum.has_value()) gemm_tc(Pi, xs, true, false, share(*dw_accum, 0, v0, n), true, kBands);
-    else if (want_dw) gemm_tc(Pi, xs, true, false, share(dw, 0, v0, n), false, kBands);
+    if (split_w) {
+      const auto pw = new_empty({sw.shares(xs.size(0)), sw.pad, H}, x, at::kFloat);
+      gemm_split_k(Pi, xs, true, pw);
+      sum_parts(pw, pw.size(0), false, V, dw_accum.has_value() ? *dw_accum : dw);
+    } else if (dw_accum.has_value()) {
+      gemm_tc(Pi, xs, true, false, share(*dw_accum, 0, v0, n), true, kBands);
+    } else if (want_dw) {
+      gemm_tc(Pi, xs, true, false, share(dw, 0, v0, n), false, kBands);
+    }
   }
-  if (parts.defined()) {
-    // (with the low rows a part holds two summands of T rows each)
-    const int64_t vecs = T * H / 4, twice = rows / T;
-    const int grid = (int)std::min<int64_t>((vecs + 255) / 256, (int64_t)num_sms() * 8);
-    launch_early(parts_sum_kernel, grid, 256, 0, reinterpret_cast<const float4*>(parts.data_ptr()), (int)(n_parts * twice),
-                 parts.size(1) / twice * H / 4, vecs, reinterpret_cast<__nv_bfloat16*>(dx.data_ptr()));
-    EMB_LAUNCH_CHECK();
-    count_launch();
-  }
+  if (parts.defined()) sum_parts(parts, n_parts, rows > T, T, dx);
   return {dx, dw};
 }
 

@@ -117,7 +117,7 @@ __device__ __forceinline__ void ce_grad_chunk(const CeRow& row, uint32_t* z, int
 }
 
 void linear_ce_gemm(const at::Tensor& x, const at::Tensor& w, const CeArgs& ce, bool grad, const at::Tensor& out);
-void gemm_split_k(const at::Tensor& a, const at::Tensor& b, const at::Tensor& parts);
+void gemm_split_k(const at::Tensor& a, const at::Tensor& b, bool trans_a, const at::Tensor& parts);
 at::Tensor gemm_tc(at::Tensor a, at::Tensor b, bool trans_a, bool trans_b, c10::optional<at::Tensor> out, bool accumulate,
                    int64_t variant);
 

@@ -47,7 +47,8 @@ def check(a, e, bound, rounded=True):
 
 
 SIZES = [(1, 1000, 64), (1, 5, 8), (3, 257, 72), (128, 513, 256), (129, 4097, 136), (250, 32001, 512), (300, 2049, 1024),
-         (1, 32000, 1024), (777, 1025, 264), (1500, 6000, 520), (64, 50001, 128)]
+         (1, 32000, 1024), (777, 1025, 264), (1500, 6000, 520), (64, 50001, 128),
+         (4000, 300, 64), (3000, 100, 72), (2500, 1000, 264), (100, 3000, 520), (128, 700, 1032)]
 
 
 @pytest.mark.parametrize("T,V,H", SIZES)
@@ -67,7 +68,8 @@ def test_against_64_bits(T, V, H):
 
 
 @pytest.mark.parametrize("T,V,H,piece", [(300, 2049, 256, 256), (300, 2049, 256, 1024), (40, 3001, 128, 512),
-                                         (2000, 5000, 512, 2048), (1, 2000, 64, 256), (700, 1281, 4096, 256)])
+                                         (2000, 5000, 512, 2048), (1, 2000, 64, 256), (700, 1281, 4096, 256),
+                                         (2600, 300, 128, 1024), (3000, 100, 72, 256), (120, 2000, 256, 512)])
 def test_pieces_main_grad_and_determinism(T, V, H, piece, monkeypatch):
     x, w, labels, dloss = make(T, V, H, seed=3)
     loss, dx, dw, bx, bw = exact(x, w, labels, dloss)
