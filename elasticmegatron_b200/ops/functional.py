@@ -442,10 +442,13 @@ def rope_qkv(qkv, cos, sin, nrot, interleaved: bool = False):
     ``cos`` / ``sin`` are fp32 [s, r/2], or [s, b, r/2] where the sequences of the batch have positions of their own
     (:func:`rope_tables` makes them); the first ``r <= d`` channels of a head turn, in the pairs (i, i + r/2) or, with
     ``interleaved``, (2i, 2i + 1).  bf16, fp16 or fp32; the result has the type of ``qkv``."""
-    _check_heads(qkv, cos, sin, nrot)
+    native = use_native(qkv)
     if (not interleaved and cos.dim() == 2 and 2 * cos.shape[-1] == qkv.shape[-1]
-            and (qkv.dtype == torch.bfloat16 or not qkv.is_cuda)):
+            and (qkv.dtype == torch.bfloat16 or not native)):
         return RoPEFn.apply(qkv, cos, sin, nrot)
+    if native:  # (the extension checks the arguments)
+        return ext().heads(qkv, None, None, cos, sin, nrot, 0, 0.0, interleaved)
+    _check_heads(qkv, cos, sin, nrot)
     return HeadsFn.apply(qkv, None, None, cos, sin, nrot, 0, 0.0, interleaved)
 
 
