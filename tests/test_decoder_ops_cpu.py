@@ -169,6 +169,11 @@ ROUTES = [  # E, k, sigmoid, bias, groups, topg, renorm
     (64, 8, True, True, 8, 4, True),
     (256, 8, True, True, 8, 4, True),
     (512, 32, True, False, 32, 32, True),
+    (64, 8, True, True, 4, 2, True),    # groups valued by four experts
+    (24, 6, False, True, 3, 2, False),  # by three, eight to a group
+    (60, 8, True, True, 4, 1, True),    # by eight, groups that are no whole lanes
+    (60, 2, False, True, 4, 1, False),
+    (320, 8, True, True, 8, 4, True),
 ]
 
 
