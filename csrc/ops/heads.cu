@@ -9,7 +9,7 @@
 //
 // Two kernels: a direct one, which holds its heads in registers (small calls, views, turns that do not fill vectors), and a
 // streamed one for the rest, both bound by memory.  Of a copy's rate at 8192 x 4 tokens, 8 x (4 + 2) heads of 128, bf16: norm
-// forward 128 us (0.97), norm backward 200 us (0.87 of the bytes' floor); rotation alone at 8192 x 2 tokens 65.6 us (0.94).
+// forward 128 us (0.97), norm backward 190 us (0.92 of the bytes' floor); rotation alone at 8192 x 2 tokens 65.6 us (0.94).
 //
 // All sums are fp32; results are rounded once, to the type of qkv.  dw is summed in a fixed order: registers, the
 // lanes of a warp, the warps of a CTA, then the CTAs' partials, so it does not change from run to run.
@@ -18,8 +18,7 @@
 // rotated pair sit in one lane: vectors (p, p + r/2/VEC) for halves, (2p, 2p + 1) for interleaved.  In both
 // layouts pair p then uses cosines [VEC p, VEC p + VEC) and no rotation needs a shuffle; only the norm's mean does.
 // VEC = 8 (16-byte accesses for 16-bit types) needs d % 8 == 0, r % 16 == 0 and aligned rows; every other shape
-// (odd quarters of a head, unaligned views) takes VEC = 1, which touches the same sectors with narrower accesses (777 x 3
-// tokens, 25 heads of 96, fp32: 14.4 us, 0.48 of a copy's rate).
+// (odd quarters of a head, unaligned views) takes VEC = 1, which touches the same sectors with narrower accesses.
 #include "../include/common.cuh"
 
 #include <c10/cuda/CUDAGuard.h>
@@ -410,6 +409,43 @@ __device__ __forceinline__ void load8(const T* p, f2* v) {
     }
   }
 }
+// 4 channels as 2 pairs
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, f2* v) {
+  if constexpr (sizeof(T) == 4) {
+    const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(p);
+    v[0] = u.x;
+    v[1] = u.y;
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const unsigned w[2] = {u.x, u.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        v[i] = f2_of(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[i] = f2_of(f.x, f.y);
+      }
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ unsigned pack2(f2 v) {
+  const float2 f = f2_to(v);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const unsigned*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    return *reinterpret_cast<const unsigned*>(&h);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const f2* v) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(v[0], v[1]);
+  else *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v[0]), pack2<T>(v[1]));
+}
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const f2* v) {
   if constexpr (sizeof(T) == 4) {
@@ -417,25 +453,12 @@ __device__ __forceinline__ void store8(T* p, const f2* v) {
     q[0] = make_ulonglong2(v[0], v[1]);
     q[1] = make_ulonglong2(v[2], v[3]);
   } else {
-    uint4 u;
-    unsigned* w = &u.x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = f2_to(v[i]);
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
-        w[i] = *reinterpret_cast<const unsigned*>(&h);
-      } else {
-        const __half2 h = __floats2half2_rn(f.x, f.y);
-        w[i] = *reinterpret_cast<const unsigned*>(&h);
-      }
-    }
-    *reinterpret_cast<uint4*>(p) = u;
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0]), pack2<T>(v[1]), pack2<T>(v[2]), pack2<T>(v[3]));
   }
 }
 
 // 4 cosines and sines from column `col` of a row of the tables
-__device__ __forceinline__ void load4(const StreamParams& p, unsigned row, int col, f2* c, f2* s) {
+__device__ __forceinline__ void load_turn(const StreamParams& p, unsigned row, int col, f2* c, f2* s) {
   const size_t at = (size_t)row * (p.r / 2) + col;
   const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(p.cosv + at), v = *reinterpret_cast<const ulonglong2*>(p.sinv + at);
   c[0] = u.x;
@@ -444,20 +467,53 @@ __device__ __forceinline__ void load4(const StreamParams& p, unsigned row, int c
   s[1] = v.y;
 }
 
-// The two vectors of 8 channels that lane `pair` holds of its head, as channel offsets, and whether each turns.
-template <bool INTER>
-__device__ __forceinline__ void vectors_of(int pair, int d, int r, int& a, int& b, bool& ta, bool& tb) {
-  if constexpr (INTER) {  // pairs lie inside a vector; neighbouring lanes take neighbouring vectors (no bank conflicts)
-    a = pair * 8;
-    b = a + (d / 8 + 1) / 2 * 8;
-    ta = a < r;
-    tb = b < r;
+// What a lane holds of its head: four quarters of 4 channels, q[i] in all.  Halves: quarter i turns with quarter i + 2 if
+// turn[i], by cosines [8 lane + 4 i, ..).  Interleaved: pairs lie inside a quarter; quarters 0 and 1 turn if turn[0], 2 and 3
+// if turn[1].  UNIT 8: quarters 0 and 1, and 2 and 3, are one aligned vector of 8 channels; UNIT 4 serves halves of r = 8 mod
+// 16 channels, where a vector of 8 would meet its partner at an offset of 4.
+struct Held {
+  int at[4];
+  bool has[4], turn[2];
+};
+template <int UNIT, bool INTER>
+__device__ __forceinline__ Held held_by(int lane, int d, int r) {
+  Held h;
+  if constexpr (UNIT == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int pair = 2 * lane + i;
+      h.turn[i] = pair < r / 8;
+      h.at[i] = h.turn[i] ? 4 * pair : r + 8 * (pair - r / 8);
+      h.at[i + 2] = h.turn[i] ? 4 * pair + r / 2 : h.at[i] + 4;
+      h.has[i] = h.has[i + 2] = pair < d / 8;
+    }
   } else {
-    const int hv = r / 16;
-    ta = tb = pair < hv;
-    a = ta ? pair * 8 : r + 2 * (pair - hv) * 8;
-    b = ta ? (pair + hv) * 8 : a + 8;
+    const int pairs = (d / 8 + 1) / 2;  // lanes past them hold nothing
+    int a, b;
+    if constexpr (INTER) {  // neighbouring lanes take neighbouring vectors (no bank conflicts)
+      a = lane * 8;
+      b = a + pairs * 8;
+      h.turn[0] = a < r;
+      h.turn[1] = b < r;
+    } else {
+      const int hv = r / 16;
+      h.turn[0] = h.turn[1] = lane < hv;
+      a = lane < hv ? lane * 8 : r + 2 * (lane - hv) * 8;
+      b = lane < hv ? (lane + hv) * 8 : a + 8;
+    }
+    h.has[0] = h.has[1] = lane < pairs && a < d;
+    h.has[2] = h.has[3] = lane < pairs && b < d;
+    h.at[0] = a;
+    h.at[1] = a + 4;
+    h.at[2] = b;
+    h.at[3] = b + 4;
   }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) h.turn[i] = h.turn[i] && h.has[INTER ? 2 * i : i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (!h.has[i]) h.at[i] = 0;
+  return h;
 }
 
 // A lane works on 16 channels of a head in packed fp32 and keeps the cosines and sines while it meets heads of one token
@@ -466,11 +522,14 @@ __device__ __forceinline__ void vectors_of(int pair, int d, int r, int& a, int& 
 // kernel from the memory's rate otherwise is the number of instructions: 4 heads of 128 channels have about 350 issue
 // slots forward and 500 backward at the rate of a plain copy; they take 196 and 308 instructions (394 and 611 in scalar
 // arithmetic, which made this kernel slower than the direct one).
-template <typename T, int LPH, int STAGES, bool INTER, bool NORM, bool BWD>
-__global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_stream_kernel(StreamParams p) {
+template <typename T, int LPH, int STAGES, int UNIT, bool INTER, bool NORM, bool BWD>
+__global__ void __launch_bounds__(kStreamWarps * 32, 2) heads_stream_kernel(StreamParams p) {
   constexpr int HPW = 32 / LPH;
   constexpr int BUFS = NORM && BWD ? 2 : 1;  // dy (or x), and x
-  constexpr bool RUNS = NORM && BWD;
+  // Tiles a warp takes in a row: the norm's backward, short of issue slots, so meets heads of one token in a row and loads its
+  // cosines and sines less often (backward of 8192 x 4 / 8192 tokens, runs of 2 / 4 / 8 / 16 tiles: 202 / 194 / 190 / 192 and
+  // 59.1 / 58.0 / 57.1 / 57.1 us; one run for all of a warp's tiles 200 to 209 and 56.0).
+  constexpr unsigned RUN = NORM && BWD ? 8 : 1;
   constexpr int kTileBytes = tile_bytes(NORM && BWD);
   extern __shared__ __align__(128) uint8_t s_ring[];
   __shared__ uint64_t s_bar[kStreamWarps][STAGES];
@@ -479,23 +538,19 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
   uint8_t* ring = s_ring + warp * (STAGES * BUFS * kTileBytes);
   uint64_t* bar = s_bar[warp];
   const unsigned head_bytes = p.d * (unsigned)sizeof(T);
-  const unsigned long long warps = (unsigned long long)gridDim.x * kStreamWarps, me = blockIdx.x * kStreamWarps + warp;
-  // the norm's backward, which is short of issue slots, takes consecutive tiles; the others walk the tensor together
-  const unsigned first = (unsigned)(RUNS ? p.tiles * me / warps : me);
-  const unsigned last = RUNS ? (unsigned)(p.tiles * (me + 1) / warps) : p.tiles, step = RUNS ? 1u : (unsigned)warps;
+  // The warps walk the tensor together, each taking RUN consecutive tiles at a time, and share what is left evenly.
+  const unsigned me = blockIdx.x * kStreamWarps + warp, warps = gridDim.x * kStreamWarps;
+  const unsigned whole = p.tiles / (warps * RUN), rest = p.tiles - whole * warps * RUN;
+  const unsigned rest0 = (unsigned)((unsigned long long)rest * me / warps);
+  const unsigned mine = whole * RUN + (unsigned)((unsigned long long)rest * (me + 1) / warps) - rest0;
+  auto tile_of = [&](unsigned it) -> unsigned {
+    return it < whole * RUN ? (it / RUN * warps + me) * RUN + it % RUN : whole * warps * RUN + rest0 + it - whole * RUN;
+  };
   const char* src0 = reinterpret_cast<const char*>(BWD ? p.dy : p.x);
   const char* src1 = reinterpret_cast<const char*>(p.x);
 
-  int oa, ob;
-  bool ta, tb;
-  vectors_of<INTER>(l, p.d, p.r, oa, ob, ta, tb);
-  const int pairs = (p.d / 8 + 1) / 2;  // lanes past them hold nothing
-  const bool ha = l < pairs && oa < p.d, hb = l < pairs && ob < p.d;
-  ta = ta && ha;
-  tb = tb && hb;
-  const bool full = pairs == LPH && p.d % 16 == 0;  // every lane holds two vectors
-  if (!ha) oa = 0;
-  if (!hb) ob = 0;
+  const Held held = held_by<UNIT, INTER>(l, p.d, p.r);
+  const bool full = LPH * 16 == p.d;  // every lane holds four quarters
 
   auto load = [&](unsigned tile, int st) {  // lane 0
     const unsigned h0 = tile * p.tile_heads, n = min(p.tile_heads, p.heads - h0), bytes = n * head_bytes;
@@ -516,20 +571,17 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
   if (lane == 0) {
 #pragma unroll
     for (int i = 0; i < STAGES; ++i)
-      if (first + (unsigned long long)i * step < last) load(first + i * step, i);
+      if (i < mine) load(tile_of(i), i);
   }
   f2 gw[NORM && BWD ? 2 : 1][8];
   if constexpr (NORM) {
     if (threadIdx.x < 2 * LPH) {  // thread (class, l) lays out that lane's weights
       const int c = threadIdx.x / LPH, q = threadIdx.x % LPH;
-      int qa, qb;
-      bool qt;
-      vectors_of<INTER>(q, p.d, p.r, qa, qb, qt, qt);
+      const Held his = held_by<UNIT, INTER>(q, p.d, p.r);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int ch = (j < 8 ? qa : qb) + (j & 7);
-        s_w[c][j / 4][q][j & 3] = q < pairs && ch < p.d ? to_f<T>(reinterpret_cast<const T*>(p.w[c])[ch]) : 0.f;
-      }
+      for (int j = 0; j < 16; ++j)
+        s_w[c][j / 4][q][j & 3] =
+            his.has[j / 4] ? to_f<T>(reinterpret_cast<const T*>(p.w[c])[his.at[j / 4] + (j & 3)]) : 0.f;
     }
 #pragma unroll
     for (int c = 0; c < (BWD ? 2 : 1); ++c)
@@ -542,8 +594,8 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
 
   unsigned from = 0x80000000u;  // first head of the table row in cs / sn (none yet)
   f2 cs[4], sn[4];
-  unsigned it = 0;
-  for (unsigned tile = first; tile < last; tile += step, ++it) {
+  for (unsigned it = 0; it < mine; ++it) {
+    const unsigned tile = tile_of(it);
     const int st = it % STAGES;
     if (!bulk_wait(bar + st, (it / STAGES) & 1)) {
       // a copy that does not arrive: report it, and leave after a bounded wait for the copies in flight
@@ -571,30 +623,37 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
       }
       const unsigned h = h0 + i;
       const bool is_k = slot >= (unsigned)p.nq;
-      T* va = reinterpret_cast<T*>(buf + i * head_bytes) + oa;
-      T* vb = reinterpret_cast<T*>(buf + i * head_bytes) + ob;
+      T* head = reinterpret_cast<T*>(buf + i * head_bytes);
       if (live && h - from >= p.per_row) {  // another row of the tables than the lane's last head had
         const unsigned row = p.rows.div(p.per_token.div(h));
         from = row * p.per_row;
         if constexpr (INTER) {
-          if (ta) load4(p, row, oa / 2, cs, sn);
-          if (tb) load4(p, row, ob / 2, cs + 2, sn + 2);
-        } else if (ta) {
-          load4(p, row, oa, cs, sn);
-          load4(p, row, oa + 4, cs + 2, sn + 2);
+          if (held.turn[0]) load_turn(p, row, held.at[0] / 2, cs, sn);
+          if (held.turn[1]) load_turn(p, row, held.at[2] / 2, cs + 2, sn + 2);
+        } else {
+          if (held.turn[0]) load_turn(p, row, held.at[0], cs, sn);
+          if (held.turn[1]) load_turn(p, row, held.at[1], cs + 2, sn + 2);
         }
       }
       f2 a[8], x[8];
-      load8<T>(va, a);
-      load8<T>(vb, a + 4);
-      if constexpr (NORM && BWD) {
-        load8<T>(va + kTileBytes / sizeof(T), x);
-        load8<T>(vb + kTileBytes / sizeof(T), x + 4);
+      if constexpr (UNIT == 8) {
+        load8<T>(head + held.at[0], a);
+        load8<T>(head + held.at[2], a + 4);
+        if constexpr (NORM && BWD) {
+          load8<T>(head + held.at[0] + kTileBytes / sizeof(T), x);
+          load8<T>(head + held.at[2] + kTileBytes / sizeof(T), x + 4);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          load4<T>(head + held.at[q], a + 2 * q);
+          if constexpr (NORM && BWD) load4<T>(head + held.at[q] + kTileBytes / sizeof(T), x + 2 * q);
+        }
       }
       if (!full) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (!(j < 4 ? ha : hb)) {
+          if (!held.has[j / 2]) {
             a[j] = 0ull;
             if (NORM && BWD) x[j] = 0ull;
           }
@@ -604,15 +663,16 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
         if constexpr (INTER) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            if (j < 4 ? ta : tb) {
+            if (held.turn[j / 4]) {
               const float2 c = f2_to(cs[j / 2]), s = f2_to(sn[j / 2]), u = f2_to(v[j]);
               const float cj = j & 1 ? c.y : c.x, sj = j & 1 ? s.y : s.x;
               v[j] = BWD ? f2_of(u.x * cj + u.y * sj, u.y * cj - u.x * sj) : f2_of(u.x * cj - u.y * sj, u.y * cj + u.x * sj);
             }
           }
-        } else if (ta) {
+        } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
+            if (!held.turn[j / 2]) continue;
             const f2 u = v[j], w = v[4 + j], neg = f2_mul(sn[j], f2_of(-1.f, -1.f));
             v[j] = f2_fma(w, BWD ? sn[j] : neg, f2_mul(u, cs[j]));
             v[4 + j] = f2_fma(u, BWD ? neg : sn[j], f2_mul(w, cs[j]));
@@ -668,8 +728,14 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
       } else {
         turn(a);
       }
-      if (live && ha) store8<T>(va, a);
-      if (live && hb) store8<T>(vb, a + 4);
+      if constexpr (UNIT == 8) {
+        if (live && held.has[0]) store8<T>(head + held.at[0], a);
+        if (live && held.has[2]) store8<T>(head + held.at[2], a + 4);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (live && held.has[q]) store4<T>(head + held.at[q], a + 2 * q);
+      }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -680,10 +746,9 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
                    : "memory");
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       // the stage of the tile before this one is free once its store has read it
-      const unsigned next = tile + (STAGES - 1) * step;  // (tiles and warps are below 2^30)
-      if (it > 0 && next < last) {
+      if (it > 0 && it + STAGES - 1 < mine) {
         asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        load(next, (it - 1) % STAGES);
+        load(tile_of(it + STAGES - 1), (it - 1) % STAGES);
       }
     }
     __syncwarp();
@@ -702,8 +767,8 @@ __global__ void __launch_bounds__(kStreamWarps * 32, NORM && BWD ? 2 : 2) heads_
           v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
           v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
         }
-        const int ch = (j < 4 ? oa : ob) + 2 * (j & 3);
-        if (sub == 0 && (j < 4 ? ha : hb)) *reinterpret_cast<float2*>(&s_dw[(warp * 2 + c) * p.d + ch]) = v;
+        const int ch = held.at[j / 2] + 2 * (j & 1);
+        if (sub == 0 && held.has[j / 2]) *reinterpret_cast<float2*>(&s_dw[(warp * 2 + c) * p.d + ch]) = v;
       }
     }
     __syncthreads();
@@ -818,8 +883,7 @@ struct Access {
 };
 
 // Fills the parameters that forward and backward share.
-Access set_up(HeadParams& p, const at::Tensor& t, const at::Tensor& cosv, const at::Tensor& sinv, int64_t nq, int64_t nk,
-              bool interleaved) {
+Access set_up(HeadParams& p, const at::Tensor& t, const at::Tensor& cosv, const at::Tensor& sinv, int64_t nq, int64_t nk) {
   TORCH_CHECK_VALUE(t.dim() == 5, "qkv must be [s, b, groups, slots, d]");
   const int64_t s = t.size(0), b = t.size(1), G = t.size(2), S = t.size(3), d = t.size(4);
   TORCH_CHECK_VALUE(nq >= 0 && nk >= 0 && nq + nk <= S, "more query and key heads than slots in a group");
@@ -844,7 +908,7 @@ Access set_up(HeadParams& p, const at::Tensor& t, const at::Tensor& cosv, const 
   p.n[1] = (int)nk;
   p.n[2] = (int)(S - nq - nk);
   const bool ok = d % 8 == 0 && (uintptr_t)p.cosv % 16 == 0 && (uintptr_t)p.sinv % 16 == 0;
-  return {ok && r % 16 == 0, ok && r % (interleaved ? 8 : 16) == 0};
+  return {ok && r % 16 == 0, ok && r % 8 == 0};
 }
 
 bool rows_aligned(const at::Tensor& t) {
@@ -869,11 +933,11 @@ int split_grid(HeadParams& p, bool vec, int waves) {
   return at;
 }
 
-template <typename T, int LPH, bool INTER, bool NORM, bool BWD>
+template <typename T, int LPH, int UNIT, bool INTER, bool NORM, bool BWD>
 void launch_stream(const StreamParams& p, int grid) {
   constexpr int kStages = 3;
   constexpr int kSmem = kStreamWarps * kStages * tile_bytes(NORM && BWD) * (NORM && BWD ? 2 : 1);
-  auto kern = heads_stream_kernel<T, LPH, kStages, INTER, NORM, BWD>;
+  auto kern = heads_stream_kernel<T, LPH, kStages, UNIT, INTER, NORM, BWD>;
   static bool done[kMaxDevices] = {};  // the shared-memory limit belongs to the device's context
   int dev = 0;
   EMB_CUDA_CHECK(cudaGetDevice(&dev));
@@ -884,32 +948,34 @@ void launch_stream(const StreamParams& p, int grid) {
   launch_early(kern, grid, kStreamWarps * 32, kSmem, p);
 }
 
+template <typename T, int LPH, int UNIT, bool INTER>
+void pick_stream_mode(const StreamParams& p, int grid, bool norm, bool bwd) {
+  if (norm) bwd ? launch_stream<T, LPH, UNIT, INTER, true, true>(p, grid) : launch_stream<T, LPH, UNIT, INTER, true, false>(p, grid);
+  else bwd ? launch_stream<T, LPH, UNIT, INTER, false, true>(p, grid) : launch_stream<T, LPH, UNIT, INTER, false, false>(p, grid);
+}
+
 template <typename T, int LPH>
-void pick_stream_mode(const StreamParams& p, int grid, bool inter, bool norm, bool bwd) {
-  if (inter) {
-    if (norm) bwd ? launch_stream<T, LPH, true, true, true>(p, grid) : launch_stream<T, LPH, true, true, false>(p, grid);
-    else bwd ? launch_stream<T, LPH, true, false, true>(p, grid) : launch_stream<T, LPH, true, false, false>(p, grid);
-  } else {
-    if (norm) bwd ? launch_stream<T, LPH, false, true, true>(p, grid) : launch_stream<T, LPH, false, true, false>(p, grid);
-    else bwd ? launch_stream<T, LPH, false, false, true>(p, grid) : launch_stream<T, LPH, false, false, false>(p, grid);
-  }
+void pick_stream_unit(const StreamParams& p, int grid, bool inter, bool norm, bool bwd) {
+  if (inter) pick_stream_mode<T, LPH, 8, true>(p, grid, norm, bwd);
+  else if (p.r % 16 == 0) pick_stream_mode<T, LPH, 8, false>(p, grid, norm, bwd);
+  else pick_stream_mode<T, LPH, 4, false>(p, grid, norm, bwd);
 }
 
 template <typename T>
 void pick_stream(const StreamParams& p, int grid, bool inter, bool norm, bool bwd) {
   switch (lanes_per_head(p.d, 8)) {
-    case 1: case 2: case 4: return pick_stream_mode<T, 4>(p, grid, inter, norm, bwd);
-    case 8: return pick_stream_mode<T, 8>(p, grid, inter, norm, bwd);
-    case 16: return pick_stream_mode<T, 16>(p, grid, inter, norm, bwd);
-    default: return pick_stream_mode<T, 32>(p, grid, inter, norm, bwd);
+    case 1: case 2: case 4: return pick_stream_unit<T, 4>(p, grid, inter, norm, bwd);
+    case 8: return pick_stream_unit<T, 8>(p, grid, inter, norm, bwd);
+    case 16: return pick_stream_unit<T, 16>(p, grid, inter, norm, bwd);
+    default: return pick_stream_unit<T, 32>(p, grid, inter, norm, bwd);
   }
 }
 
 // Dense tensors with 16-byte rows are streamed from a number of heads up, below which the rings' start costs more than the
 // loads that they hide.  Heads of 128, groups of 4 + 2, in L2, direct / streamed: forward 24576 heads 4.7 / 5.6 us, 49152
 // 7.4 / 7.3, 98304 11.8 / 11.2; backward with norm 12288 heads 9.0 / 8.6, 24576 13.2 / 11.5, 49152 19.2 / 14.4 (heads of 64
-// and single-head groups cross at 24576 to 49152 too).  They are streamed at any size where the interleaved turn
-// ends in the middle of the direct kernel's 16-channel pairs (r = 8 mod 16; the direct kernel would go by single channels).
+// and single-head groups cross at 24576 to 49152 too).  They are streamed at any size where r = 8 mod 16, which
+// the direct kernel would take by single channels.
 bool streams(const HeadParams& p, Access a, const at::Tensor& t, const at::Tensor& other) {
   const long long heads = p.tokens * p.G * p.S, from = other.defined() ? 24576 : 49152;  // (other: the norm's backward)
   return (a.direct ? heads >= from : a.stream) && t.is_contiguous() &&
@@ -984,7 +1050,7 @@ at::Tensor heads_fwd(at::Tensor qkv, at::Tensor cosv, at::Tensor sinv, int64_t n
   const c10::cuda::CUDAGuard guard(qkv.device());
   HeadParams p{};
   const bool norm = wq.has_value();
-  Access vec = set_up(p, qkv, cosv, sinv, nq, nk, interleaved);
+  Access vec = set_up(p, qkv, cosv, sinv, nq, nk);
   auto x = inner_contiguous(qkv);
   if (norm) {
     check_weights(wq, x, "q_weight");
@@ -1025,7 +1091,7 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
   const c10::cuda::CUDAGuard guard(dy.device());
   HeadParams p{};
   const bool norm = wq.has_value();
-  Access vec = set_up(p, dy, cosv, sinv, nq, nk, interleaved);
+  Access vec = set_up(p, dy, cosv, sinv, nq, nk);
   auto g = inner_contiguous(dy);
   at::Tensor x;
   if (norm) {

@@ -53,6 +53,10 @@ HEADS = [  # s, b, G, hpg, d, r, per_seq
     (901, 3, 6, 2, 80, 80, True),
     (700, 1, 8, 8, 256, 256, False),
     (13, 1, 2, 1, 96, 24, False),
+    (1500, 2, 8, 4, 96, 24, False),  # turns of 8 mod 16 channels
+    (801, 3, 6, 2, 80, 40, True),
+    (40, 1, 3, 1, 72, 8, False),
+    (6, 2, 1, 2, 512, 264, False),
     (3, 1, 1, 2, 64, 0, False),     # nothing turns
 ]
 
