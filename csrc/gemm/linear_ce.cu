@@ -6,8 +6,8 @@
 // backward, per piece [v0, v1) of the vocabulary, with P = (softmax(z) - onehot) dloss of that piece only:
 //           product again with the gradient epilogue -> P (bf16);   dx += P w[v0:v1] (fp32);   dw[v0:v1] (+)= P^T x.
 //           6 T V H operations: 2 more than with kept logits.
-// 8192 x 129024 x 4096: forward 5.2 ms (1654 TFLOP/s before the power limit), a whole step 25.5 ms, 8 T V H at 1357
-// TFLOP/s (the library's sustained rate: 1358); 4096 x 32000 x 4096: 3.27 ms; 250 x 32001 x 512: 76 us.
+// 8192 x 129024 x 4096: forward 5.2 ms (1654 TFLOP/s before the power limit), a whole step 25.8 ms, 8 T V H at 1343
+// TFLOP/s (the library's sustained rate: 1358); 4096 x 32000 x 4096: 3.23 ms; 250 x 32001 x 512: 76 us.
 //
 // P is rounded to bf16 because the tensor cores multiply bf16; everything summed over V or T is summed in fp32.  With
 // many rows these roundings average out next to that of the result.  With few, one entry, the label's, can be all there is
