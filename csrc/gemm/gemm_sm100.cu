@@ -926,7 +926,6 @@ __global__ void __launch_bounds__(AG ? NUM_THREADS_AG : NUM_THREADS, 1)
         TMEM_LD_32(taddr, r);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         const int col0 = n0 + c * 32;
-        if constexpr (EPI == kCeGrad) ce_grad_chunk(ce_row, r, col0);  // by the whole warp
         if (!row_ok || col0 >= p.N || p.no_store) continue;
         const int ncols = min(32, p.N - col0);
         void* gdst;
@@ -1143,7 +1142,10 @@ static void launch(int bk, const CUtensorMap& tA, const CUtensorMap& tB, const C
   int dev = 0;
   EMB_CUDA_CHECK(cudaGetDevice(&dev));
   const int which = bk == 128 ? 1 : 0;
-  auto kern = which ? gemm2_kernel<AG, 128, EPI> : gemm2_kernel<AG, 64, EPI>;
+  auto kern = gemm2_kernel<AG, 128, EPI>;
+  if constexpr (EPI == gk::kStore) {
+    if (!which) kern = gemm2_kernel<AG, 64, EPI>;
+  }
   const int smem = which ? smem_bytes<128>() : smem_bytes<64>();
   if (!attr_set[which][dev]) {
     EMB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -1384,7 +1386,10 @@ void linear_ce_gemm(const at::Tensor& x, const at::Tensor& w, const CeArgs& ce, 
     CUtensorMap tA = make_map(x.data_ptr(), M, K, x.stride(0), 64, 128), tB = make_map(w.data_ptr(), N, K, w.stride(0), 64, 128);
     CUtensorMap tC = tA;
     p.split_tail = grad ? 1 : 0;  // the statistics have one slot for each whole tile
-    if (grad) p.c_tma = make_c_map(out, false, M, N, tC) ? 1 : 0;
+    if (grad) {
+      TORCH_CHECK(make_c_map(out, false, M, N, tC), "linear cross entropy: gradient buffer must be 16-byte aligned");
+      p.c_tma = 1;
+    }
     const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
     const int clusters = (int)std::min<int64_t>(tiles, num_sms() / 2);
     if (grad) gk2::launch<false, kCeGrad>(128, tA, tB, tC, p, clusters, true);
