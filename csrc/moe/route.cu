@@ -41,6 +41,9 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr float kTiny = 1e-20f;
 constexpr int kRouteWarps = 16;
 constexpr int kMaxExperts = 512, kMaxTopk = 32, kMaxGroups = 32;
+// The most shared memory that a forward asks for: 16 experts a lane (keys and scores of 512), counts, and the rows of 32
+// groups of up to 16 experts at a stride of 33 words.
+constexpr int kRouteSmem = (2 * kRouteWarps * 32 * 16 + kMaxExperts + kRouteWarps * kMaxGroups * 33) * 4;
 
 struct RouteParams {
   const void* logits;
@@ -602,7 +605,7 @@ std::vector<at::Tensor> moe_route_fwd(at::Tensor logits, int64_t k, bool sigmoid
       static bool done[kMaxDevices] = {};  // the limit belongs to the device's context
       int dev = 0;
       EMB_CUDA_CHECK(cudaGetDevice(&dev));
-      if (!done[dev]) EMB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
+      if (!done[dev]) EMB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteSmem));
       done[dev] = true;
     }
     launch_early(kern, grid, kRouteWarps * 32, smem, p);
