@@ -605,10 +605,17 @@ __global__ void rope_kernel(const __nv_bfloat16* __restrict__ in, __nv_bfloat16*
 
 at::Tensor rope_fwd(at::Tensor qkv, at::Tensor cosv, at::Tensor sinv, int64_t nrot, bool inverse) {
   check_cuda_bf16(qkv, "qkv");
-  TORCH_CHECK(qkv.dim() == 5, "qkv must be [s, b, G, slots, d]");
+  TORCH_CHECK_VALUE(qkv.dim() == 5, "qkv must be [s, b, G, slots, d]");
   const int64_t s = qkv.size(0), b = qkv.size(1), G = qkv.size(2), S = qkv.size(3), d = qkv.size(4);
   TORCH_CHECK(d % 16 == 0, "head dim must be a multiple of 16");
-  TORCH_CHECK(cosv.is_cuda() && cosv.scalar_type() == at::kFloat && cosv.size(0) == s && cosv.size(1) == d / 2);
+  TORCH_CHECK_VALUE(nrot >= 0 && nrot <= S, "more turned heads than slots in a group");
+  for (const auto& t : {cosv, sinv}) {
+    TORCH_CHECK(t.is_cuda() && t.device() == qkv.device() && t.scalar_type() == at::kFloat && t.is_contiguous(),
+                "cos and sin must be contiguous fp32 tensors on the device of qkv");
+    TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == s && t.size(1) == d / 2, "cos and sin must be [s, d/2]");
+  }
+  // a contiguous view may start off the 16-byte grid of the kernel's vectors
+  if (reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 != 0) qkv = qkv.clone();
   auto out = at::empty_like(qkv);
   int64_t n = s * b * G * S * (d / 16);
   if (n == 0) return out;

@@ -439,16 +439,17 @@ def rope_qkv(qkv, cos, sin, nrot, interleaved: bool = False):
     """Rotary positions of the first ``nrot`` slots (query heads and the key head) of each group of the fused
     activations ``qkv`` [s, b, G, slots, d]; the other slots pass through.
 
-    ``cos`` / ``sin`` are fp32 [s, r/2], or [s, b, r/2] where the sequences of the batch have positions of their own
+    ``cos`` / ``sin`` are dense fp32 [s, r/2], or [s, b, r/2] where the sequences of the batch have positions of their own
     (:func:`rope_tables` makes them); the first ``r <= d`` channels of a head turn, in the pairs (i, i + r/2) or, with
     ``interleaved``, (2i, 2i + 1).  bf16, fp16 or fp32; the result has the type of ``qkv``."""
     native = use_native(qkv)
+    if not native:  # (the extension checks the arguments of CUDA calls)
+        _check_heads(qkv, cos, sin, nrot)
     if (not interleaved and cos.dim() == 2 and 2 * cos.shape[-1] == qkv.shape[-1]
-            and (qkv.dtype == torch.bfloat16 or not native)):
+            and (not native or (qkv.dtype == torch.bfloat16 and qkv.shape[-1] % 16 == 0))):
         return RoPEFn.apply(qkv, cos, sin, nrot)
-    if native:  # (the extension checks the arguments)
+    if native:
         return ext().heads(qkv, None, None, cos, sin, nrot, 0, 0.0, interleaved)
-    _check_heads(qkv, cos, sin, nrot)
     return HeadsFn.apply(qkv, None, None, cos, sin, nrot, 0, 0.0, interleaved)
 
 
