@@ -76,7 +76,11 @@ __global__ void __launch_bounds__(1024) ce_join_kernel(CeArgs ce, const __nv_bfl
   out_top[t] = top;
   out_sum[t] = s;
   float z = s;
-  if (own) z = fmaxf(s - __expf(ce.target[t] - top), 0.f) + __expf(dot - top);
+  if (own) {
+    float rest = s - __expf(ce.target[t] - top);
+    if (rest < 0.f) rest = 0.f;  // (a NaN stays: fmaxf would drop it, and with it a diverged weight from every loss)
+    z = rest + __expf(dot - top);
+  }
   // a rank's share of the vocabulary leaves the label's logit and the sum that belongs to it, for the caller to join
   if (raw) out_loss_sum[t] = z;
   out[t] = !own ? 0.f : raw ? dot : logf(z) + (top - dot);

@@ -1,0 +1,27 @@
+"""Linear cross entropy kernels (csrc/gemm/linear_ce.cu) in rarer uses."""
+import math
+
+import pytest
+import torch
+
+from elasticmegatron_b200.ops import functional as F_
+from elasticmegatron_b200.ops.native import ext
+from test_linear_ce_gpu import make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("T", [20, 300])
+def test_nan_in_a_row_of_w(T):
+    """A NaN in a row of w is in every token's sum, whichever label the token has; ignored tokens keep loss 0."""
+    x, w, labels, _ = make(T, 1000, 64, seed=1)
+    w[777] = math.nan
+    labels[labels == 777] = 5
+    labels[0] = 777
+    counts = (labels >= 0) & (labels < 1000)
+    loss = F_.linear_cross_entropy(x, w, labels)
+    assert bool(torch.isnan(loss[counts]).all()) and loss[~counts].abs().sum() == 0
+    # a rank's share of the vocabulary passes it on in both sums, the other rank's share is unaffected
+    for lo, hi, bad in ((0, 512, False), (512, 1000, True)):
+        target, top, total, loss_total = ext().linear_ce_fwd(x, w[lo:hi], labels, lo, 1000, -100, True)
+        assert bool((torch.isnan(total) == bad).all()) and bool((torch.isnan(loss_total) == bad).all())
