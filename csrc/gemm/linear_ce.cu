@@ -198,8 +198,11 @@ std::vector<at::Tensor> linear_ce_fwd(at::Tensor x, at::Tensor w, at::Tensor lab
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t T = x.size(0), V = w.size(0);
   TORCH_CHECK(V > 0 && col0 >= 0 && col0 + V <= vocab && (raw || V == vocab), "columns outside the vocabulary");
-  auto out = new_empty({raw ? 4 : 3, T}, x, at::kFloat);
-  if (T == 0) return out.unbind(0);
+  // the loss (or the label's logit) has memory of its own: a caller may change it in place while the statistics are kept
+  auto out = new_empty({T}, x, at::kFloat);
+  auto stats = new_empty({raw ? 3 : 2, T}, x, at::kFloat).unbind(0);
+  stats.insert(stats.begin(), out);
+  if (T == 0) return stats;
   const int64_t tiles = (V + 255) / 256;
   auto part = new_empty({tiles * T * 2 + T}, x, at::kFloat);  // and the labels' logits
   CeArgs ce = ce_args(labels, col0, vocab, ignore);
@@ -207,14 +210,14 @@ std::vector<at::Tensor> linear_ce_fwd(at::Tensor x, at::Tensor w, at::Tensor lab
   ce.target = part.data_ptr<float>() + tiles * T * 2;
   auto xr = tma_rows(x), wr = tma_rows(w);
   linear_ce_gemm(xr, wr, ce, false, at::Tensor());
-  float* o = out.data_ptr<float>();
+  float* o = stats[1].data_ptr<float>();
   launch_early(
       ce_join_kernel, (int)((T + 31) / 32), 1024, 0, ce, reinterpret_cast<const __nv_bfloat16*>(xr.data_ptr()), xr.stride(0),
-      reinterpret_cast<const __nv_bfloat16*>(wr.data_ptr()), wr.stride(0), (int)x.size(1), (int)T, (int)tiles, (int)V, raw, o,
-      o + T, o + 2 * T, raw ? o + 3 * T : nullptr);
+      reinterpret_cast<const __nv_bfloat16*>(wr.data_ptr()), wr.stride(0), (int)x.size(1), (int)T, (int)tiles, (int)V, raw,
+      out.data_ptr<float>(), o, o + T, raw ? o + 2 * T : nullptr);
   EMB_LAUNCH_CHECK();
   count_launch();
-  return out.unbind(0);
+  return stats;
 }
 
 // {dx [T, H] bf16, dw [V, H] bf16}, each undefined where it is not wanted; with `dw_accum` (fp32 [V, H]) the weight

@@ -25,3 +25,37 @@ def test_nan_in_a_row_of_w(T):
     for lo, hi, bad in ((0, 512, False), (512, 1000, True)):
         target, top, total, loss_total = ext().linear_ce_fwd(x, w[lo:hi], labels, lo, 1000, -100, True)
         assert bool((torch.isnan(total) == bad).all()) and bool((torch.isnan(loss_total) == bad).all())
+
+
+@pytest.mark.parametrize("main", [False, True])
+@pytest.mark.parametrize("T", [20, 300])
+def test_loss_changes_in_place(T, main):
+    """The loss is a tensor of its own: scaled, masked and filled in place as any other, without touching what the
+    backward pass has kept."""
+    x, w, labels, _ = make(T, 1000, 64, seed=2)
+    mask = (torch.arange(T, device="cuda") % 3 > 0).float()
+    grads = []
+    for inplace in (False, True):
+        xi, p = x.clone().requires_grad_(), torch.nn.Parameter(w.clone())
+        if main:
+            p.main_grad = torch.zeros(1000, 64, device="cuda")
+        loss = F_.linear_cross_entropy(xi, p, labels)
+        if inplace:
+            loss *= mask
+            loss /= 2.0
+            loss.masked_fill_(labels < 0, 0.0)
+        else:
+            loss = torch.where(labels < 0, 0.0, loss * mask / 2.0)
+        loss.sum().backward()
+        grads.append((loss.detach(), xi.grad, p.main_grad if main else p.grad))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+    # without gradients, and after the pass that kept the statistics
+    xi = x.clone().requires_grad_()
+    loss = F_.linear_cross_entropy(xi, w, labels)
+    with torch.no_grad():
+        loss.zero_()
+    loss.sum().backward()
+    xj = x.clone().requires_grad_()
+    F_.linear_cross_entropy(xj, w, labels).sum().backward()
+    assert torch.equal(xi.grad, xj.grad)
