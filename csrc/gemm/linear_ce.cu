@@ -247,11 +247,11 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
     return {dx, dw};
   }
   auto xr = tma_rows(x), wr = tma_rows(w);
+  const int64_t rows = T <= 128 ? 2 * T : T;  // of P
   const int64_t whole = (V + 255) / 256 * 256;
-  if (piece <= 0) piece = kPieceBytes / (2 * T);
+  if (piece <= 0) piece = kPieceBytes / (2 * rows);
   piece = std::min(whole, std::max<int64_t>(256, piece / 256 * 256));
   const int64_t pieces = (V + piece - 1) / piece;
-  const int64_t rows = T <= 128 ? 2 * T : T;  // of P
   auto P = new_empty({rows, piece}, x, at::kBFloat16);
   const bool wants_w = want_dw || dw_accum.has_value();
   auto xs = rows > T && wants_w ? at::cat({xr, xr}) : xr;
@@ -261,14 +261,18 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
   ce.low_row = rows > T ? (int)T : 0;
   ce.dloss = g.data_ptr<float>();
   // dx of few rows and dw of few words have few output tiles and a long sum: it is split, fp32 parts joined in order
-  // (dx of 512 x 129024 x 4096: 572 -> 436 us, dw of 8192 x 1000 x 512: 82 -> 26 us against whole sums on single SMs)
+  // (dx of 512 x 129024 x 4096: 572 -> 436 us, dw of 8192 x 1000 x 512: 82 -> 26 us against whole sums on single SMs).
+  // The parts of a product fill the SMs once (a 128 x 256 tile each) and are joined before the next product.  A piece that
+  // would be one part is added to the sum by the product itself.
   const Split sx(rows, H), sw(std::min(piece, V), H);
-  const bool split = want_dx && (rows > T || (sx.pair ? sx.tiles : sx.tiles * 2) <= sx.slots);
+  const bool split = want_dx && (rows > T || ((sx.pair ? sx.tiles : sx.tiles * 2) <= sx.slots &&
+                                              (pieces == 1 || sx.shares(piece) > 1)));
   const bool split_w = wants_w && pieces == 1 && sw.shares(xs.size(0)) > 1;
-  const int64_t n_parts = split ? (pieces - 1) * sx.shares(piece) + sx.shares(V - (pieces - 1) * piece) : 1;
-  at::Tensor parts;
-  if (want_dx && (split || pieces > 1)) parts = new_empty({n_parts, split ? sx.pad : T, H}, x, at::kFloat);
-  int64_t part = 0;
+  at::Tensor total;  // dx over several pieces
+  if (want_dx && pieces > 1) {
+    total = new_empty({1, T, H}, x, at::kFloat);
+    if (split) total.zero_();
+  }
   for (int64_t i = 0; i < pieces; ++i) {
     const int64_t v0 = i * piece, n = std::min(piece, V - v0);
     const auto Pi = share(P, 1, 0, n), wi = share(wr, 0, v0, n);
@@ -276,10 +280,11 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
     linear_ce_gemm(xr, wi, ce, true, Pi);
     if (want_dx) {
       if (split) {
-        gemm_split_k(Pi, wi, false, share(parts, 0, part, sx.shares(n)));
-        part += sx.shares(n);
+        const auto px = new_empty({sx.shares(n), sx.pad, H}, x, at::kFloat);
+        gemm_split_k(Pi, wi, false, px);
+        sum_parts(px, px.size(0), rows > T, T, pieces > 1 ? total[0] : dx);
       } else {
-        gemm_tc(Pi, wi, false, false, pieces > 1 ? parts[0] : dx, i > 0, kBands);
+        gemm_tc(Pi, wi, false, false, pieces > 1 ? total[0] : dx, i > 0, kBands);
       }
     }
     if (split_w) {
@@ -292,7 +297,7 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
       gemm_tc(Pi, xs, true, false, share(dw, 0, v0, n), false, kBands);
     }
   }
-  if (parts.defined()) sum_parts(parts, n_parts, rows > T, T, dx);
+  if (total.defined()) sum_parts(total, 1, false, T, dx);
   return {dx, dw};
 }
 

@@ -730,8 +730,10 @@ def linear_cross_entropy(x, w, labels, vocab_start: int = 0, mode: Optional[str]
 
     ``x`` [T, H] and ``w`` [V, H] (bf16 on CUDA, H a multiple of 8), ``labels`` int64 [T] of global ids.  The forward
     product keeps the softmax statistics alone; the backward computes the logits again, a piece of the vocabulary at a
-    time (``LINEAR_CE_PIECE`` columns).  Memory beside the gradients: T V / 32 bytes of statistics in the forward, a bf16
-    [T, piece] buffer (256 MiB by default) and an fp32 [T, H] sum in the backward.  It costs 8 T V H
+    time (``LINEAR_CE_PIECE`` columns).  Memory: T V / 32 bytes of statistics in the forward; in the backward, beside the
+    gradients, the bf16 gradient of a piece's logits [T, piece] (256 MiB by default, 256 columns at least; two rows a token
+    up to 128 tokens, and x twice then), an fp32 [T, H] sum where there are several pieces or dx's sum is split, and 20 MB
+    of parts of a split sum at most.  It costs 8 T V H
     operations a step where :func:`linear` followed by :func:`vocab_parallel_cross_entropy` costs 6.
 
     Labels equal to ``ignore_index``, and any outside the vocabulary, have loss and gradient 0.  The weight gradient

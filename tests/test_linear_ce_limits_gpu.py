@@ -59,3 +59,28 @@ def test_loss_changes_in_place(T, main):
     xj = x.clone().requires_grad_()
     F_.linear_cross_entropy(xj, w, labels).sum().backward()
     assert torch.equal(xi.grad, xj.grad)
+
+
+@pytest.mark.parametrize("T,H,V,piece", [(1024, 1024, 16384, 256), (100, 1024, 16384, 256), (2048, 512, 32768, 4096),
+                                         (100, 512, 32768, 0), (1500, 1024, 2048, 0)])
+def test_backward_memory(T, H, V, piece, monkeypatch):
+    """Beside the gradients: a bf16 [rows, piece] buffer, one fp32 [T, H] sum and, where a product is split over the
+    SMs, one fp32 part of 128 x 256 for each of them.  Smaller pieces take less, not more."""
+    monkeypatch.setattr(F_, "LINEAR_CE_PIECE", piece)
+    x, w, labels, dloss = make(T, V, H, seed=4)
+    x.requires_grad_(), w.requires_grad_()
+    loss = F_.linear_cross_entropy(x, w, labels)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    start = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(loss, [x, w], dloss)
+    torch.cuda.synchronize()
+    used = torch.cuda.max_memory_allocated() - start
+    rows = 2 * T if T <= 128 else T
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    bound = 2 * (T + V) * H + 2 * rows * min(piece or V, V) + 4 * T * H + 4 * sms * 128 * 256
+    if T <= 128:
+        bound += 2 * rows * H  # x twice, for the product with both rows of a token
+    # small vectors, and what the allocator rounds each block up to (2 MB for blocks over 1 MB)
+    assert used <= bound + 6 * 2 ** 21, (used, bound)
+    assert len(grads) == 2
