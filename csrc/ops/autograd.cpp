@@ -33,6 +33,14 @@ bool tracks(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
 at::Tensor or_none(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
 OptTensor given(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
+// The nodes have no forward-mode rule: an input with a tangent is refused, or its derivative would silently be zero.
+template <typename... T>
+void no_tangents(const T&... inputs) {
+  for (const at::Tensor& t : {at::Tensor(inputs)...})
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
+                                "this operator does not support forward-mode differentiation");
+}
+
 // A node whose inputs are `inputs`, in the order of the gradients that apply() returns.
 template <typename N, typename... T>
 std::shared_ptr<N> new_node(const T&... inputs) {
@@ -108,12 +116,13 @@ struct LinearCeNode : torch::autograd::Node {
 
 at::Tensor heads(at::Tensor qkv, OptTensor wq, OptTensor wk, at::Tensor cosv, at::Tensor sinv, int64_t nq, int64_t nk,
                  double eps, bool interleaved) {
+  const auto q = or_none(wq), k = or_none(wk);
+  no_tangents(qkv, q, k, cosv, sinv);
   at::Tensor out;
   {
     at::NoGradGuard no_grad;
     out = heads_fwd(qkv, cosv, sinv, nq, nk, interleaved, wq, wk, eps);
   }
-  const auto q = or_none(wq), k = or_none(wk);
   if (at::GradMode::is_enabled() && (tracks(qkv) || tracks(q) || tracks(k))) {
     auto n = new_node<HeadsNode>(qkv, q, k);
     if (q.defined()) {  // the rotation alone needs no input for its gradient
@@ -134,6 +143,7 @@ at::Tensor heads(at::Tensor qkv, OptTensor wq, OptTensor wk, at::Tensor cosv, at
 
 std::vector<at::Tensor> moe_route(at::Tensor logits, OptTensor bias, int64_t k, bool sigmoid, int64_t groups, int64_t topg,
                                   bool renorm, double scaling) {
+  no_tangents(logits, or_none(bias));
   std::vector<at::Tensor> r;
   {
     at::NoGradGuard no_grad;
@@ -153,6 +163,7 @@ std::vector<at::Tensor> moe_route(at::Tensor logits, OptTensor bias, int64_t k, 
 }
 
 at::Tensor linear_ce(at::Tensor x, at::Tensor w, at::Tensor labels, int64_t ignore, int64_t piece) {
+  no_tangents(x, w);
   std::vector<at::Tensor> r;
   {
     at::NoGradGuard no_grad;
