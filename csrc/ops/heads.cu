@@ -785,11 +785,11 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2) heads_stream_kernel(Stre
 // thread has two or three loads to wait for at once; slices are joined by a fixed tree.
 template <typename T>
 __global__ void __launch_bounds__(1024) heads_join_kernel(const float* __restrict__ part, int d, int nb0, int nb1, int both,
-                                                          T* dw0, T* dw1, float* acc0, float* acc1) {
+                                                          int first, T* dw0, T* dw1, float* acc0, float* acc1) {
   __shared__ float sh[32][9];
   grid_dependency();
   // rows of `part`: those of class 0 and then those of class 1, or (`both`) the two of each block side by side
-  const int cls = blockIdx.y, by = both ? 2 : 1;
+  const int cls = first + blockIdx.y, by = both ? 2 : 1;
   const int b0 = both ? 0 : cls ? nb0 : 0, b1 = both ? nb0 : cls ? nb0 + nb1 : nb0, shift = both ? cls : 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 8 + (lane & 7);
   float v = 0.f;
@@ -1147,17 +1147,21 @@ std::vector<at::Tensor> heads_bwd(at::Tensor dy, c10::optional<at::Tensor> qkv, 
     part = new_empty({nb0 + nb1, p.d}, g, at::kFloat);
     p.part = q.part = part.data_ptr<float>();
   }
+  const bool same = acc[0] && acc[1] && acc[0] < acc[1] + p.d && acc[1] < acc[0] + p.d;
+  const int joins = !norm ? 0 : same ? 2 : 1;
   by_type(g.scalar_type(), [&](auto t) {
     using T = decltype(t);
     if (stream) pick_stream<T>(q, grid, interleaved, norm, true);
     else pick_shape<T>(p, grid, vec.direct, interleaved, norm, true);
     if (norm) {
-      launch_early(heads_join_kernel<T>, dim3((p.d + 7) / 8, 2), 1024, 0, p.part, p.d, nb0, nb1, (int)stream, (T*)dw[0],
-                   (T*)dw[1], acc[0], acc[1]);
+      // one launch for both classes, or one after the other where they add to the same words (one weight for both)
+      for (int c = 0; c < joins; ++c)
+        launch_early(heads_join_kernel<T>, dim3((p.d + 7) / 8, joins == 2 ? 1 : 2), 1024, 0, p.part, p.d, nb0, nb1,
+                     (int)stream, c, (T*)dw[0], (T*)dw[1], acc[0], acc[1]);
     }
   });
   EMB_LAUNCH_CHECK();
-  count_launch(norm ? 2 : 1);
+  count_launch(1 + joins);
   return res;
 }
 

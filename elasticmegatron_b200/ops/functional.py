@@ -415,8 +415,8 @@ class HeadsFn(torch.autograd.Function):
                 if m is not None:
                     m.view(-1).add_(g)
             dwq, dwk = dwq.to(wq.dtype), dwk.to(wk.dtype)
-        for w, m in ((wq, mq), (wk, mk)):
-            if m is not None and getattr(w, "_grad_ready", None) is not None:
+        for w in (wq,) if wk is wq else (wq, wk):  # (one weight for both is ready once)
+            if getattr(w, "main_grad", None) is not None and getattr(w, "_grad_ready", None) is not None:
                 w._grad_ready()
         return (dx, dwq if mq is None else None, dwk if mk is None else None) + none
 
