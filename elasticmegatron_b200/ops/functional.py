@@ -461,6 +461,8 @@ def qk_norm_rope_qkv(qkv, q_weight, k_weight, cos, sin, eps, interleaved: bool =
     in fp32 into ``main_grad`` where the parameters have one.  Tables and layouts as for :func:`rope_qkv`."""
     if qkv.dim() == 5 and qkv.shape[3] < 3:
         raise ValueError("a group needs at least one query head, the key head and the value head")
+    if q_weight is None or k_weight is None:
+        raise ValueError("the query and the key heads need a weight each (rope_qkv turns without a norm)")
     if use_native(qkv) and qkv.dim() == 5 and not hasattr(q_weight, "main_grad") and not hasattr(k_weight, "main_grad"):
         return ext().heads(qkv, q_weight, k_weight, cos, sin, qkv.shape[3] - 2, 1, eps, interleaved)
     _check_heads(qkv, cos, sin, qkv.shape[3] - 1 if qkv.dim() == 5 else 0)
