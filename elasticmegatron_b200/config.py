@@ -70,13 +70,6 @@ class ModelConfig:
     max_tensor_parallel_size: int = 8
     seq_length: int = 512
     rotary_base: float = 10000.0
-    # share of each head's channels that turn, pairs side by side (GPT-J) instead of in halves, and how frequencies are
-    # stretched to longer contexts (Megatron's --rotary-percent, --rotary-interleaved, --use-rope-scaling)
-    rotary_percent: float = 1.0
-    rotary_interleaved: bool = False
-    rope_scaling: Optional[RopeScaling] = None
-    # RMSNorm of every query and key head before the rotation (Megatron's --qk-layernorm)
-    qk_layernorm: bool = False
     norm_epsilon: float = 1e-5
     # "RMSNorm" (Llama) or "LayerNorm" (Megatron's default, with a bias per norm: the reference's demo model)
     normalization: str = "RMSNorm"
@@ -87,6 +80,16 @@ class ModelConfig:
     moe_router_topk: int = 2
     moe_aux_loss_coeff: float = 1e-2
     moe_ffn_hidden_size: Optional[int] = None
+    # numerics
+    params_dtype: str = "bf16"  # "bf16" | "fp32"
+    # (options added later stand behind, so that positional arguments keep their meaning)
+    # share of each head's channels that turn, pairs side by side (GPT-J) instead of in halves, and how frequencies are
+    # stretched to longer contexts (Megatron's --rotary-percent, --rotary-interleaved, --use-rope-scaling)
+    rotary_percent: float = 1.0
+    rotary_interleaved: bool = False
+    rope_scaling: Optional[RopeScaling] = None
+    # RMSNorm of every query and key head before the rotation (Megatron's --qk-layernorm)
+    qk_layernorm: bool = False
     # router: softmax after top-k, or (pre_softmax) the softmax over all experts kept as it is, or sigmoid scores divided
     # by their sum; experts limited to the best group_topk of num_groups groups; weights times topk_scaling_factor
     moe_router_score_function: str = "softmax"
@@ -94,8 +97,6 @@ class ModelConfig:
     moe_router_num_groups: Optional[int] = None
     moe_router_group_topk: Optional[int] = None
     moe_router_topk_scaling_factor: Optional[float] = None
-    # numerics
-    params_dtype: str = "bf16"  # "bf16" | "fp32"
 
     def __post_init__(self):
         if self.num_query_groups is None:
