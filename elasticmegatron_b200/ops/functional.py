@@ -738,6 +738,10 @@ def linear_cross_entropy(x, w, labels, vocab_start: int = 0, mode: Optional[str]
     of parts of a split sum at most.  It costs 8 T V H
     operations a step where :func:`linear` followed by :func:`vocab_parallel_cross_entropy` costs 6.
 
+    The loss is computed in fp32.  On CUDA the gradient of the logits is rounded to bf16 for the products, as it is with
+    kept logits: ``dx`` and ``dw`` then have about 1.4 times the relative error of their own rounding to bf16.  Up to 128
+    tokens it keeps 16 bits and that error is gone.
+
     Labels equal to ``ignore_index``, and any outside the vocabulary, have loss and gradient 0.  The weight gradient
     accumulates in fp32 into ``main_grad`` where the weight has one.  With a tensor-parallel ``group`` the weight is this
     rank's rows ``[vocab_start, vocab_start + V)`` (equal shares) and ``mode`` is that of the output layer: ``"col"`` or,

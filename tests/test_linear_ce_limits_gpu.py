@@ -6,7 +6,7 @@ import torch
 
 from elasticmegatron_b200.ops import functional as F_
 from elasticmegatron_b200.ops.native import ext
-from test_linear_ce_gpu import make
+from test_linear_ce_gpu import exact, make
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +84,19 @@ def test_backward_memory(T, H, V, piece, monkeypatch):
     # small vectors, and what the allocator rounds each block up to (2 MB for blocks over 1 MB)
     assert used <= bound + 6 * 2 ** 21, (used, bound)
     assert len(grads) == 2
+
+
+@pytest.mark.parametrize("T", [40, 128, 129, 700])
+def test_error_of_the_gradients(T):
+    """Relative error (2-norms) of dx and dw against rounding the exact gradients to bf16 alone.  Rounding each term of a
+    sum of terms of random signs costs as much again, independently: a factor of 2^1/2, of which up to 128 tokens
+    2^-8 of the second summand is left.  5 % for the fp32 sums and the chance in both figures."""
+    V, H = 6000, 256
+    x, w, labels, _ = make(T, V, H, seed=6, ignore=False)
+    dloss = torch.full((T,), 1.0 / T, device="cuda")
+    _, dx, dw, _, _ = exact(x, w, labels, dloss)
+    x.requires_grad_(), w.requires_grad_()
+    got = torch.autograd.grad(F_.linear_cross_entropy(x, w, labels), [x, w], dloss)
+    for a, e in zip(got, (dx, dw)):
+        rel = float((a.double() - e).norm()) / float((e.bfloat16().double() - e).norm())
+        assert rel < 1.05 * (1.0 if T <= 128 else math.sqrt(2.0)), rel
