@@ -15,7 +15,9 @@
 // masked in the selection (so every index stays in range) and makes the row's softmax scores NaN.
 //
 // The scores use expf and IEEE division, and the softmax sum is held in 64 bits, so s, c and with them the choice
-// are the same for every order of summation: ranks, batch splits and the host implementation agree on them.
+// are the same for every order of summation: ranks and batch splits agree on them bit for bit.  The host form takes the
+// same steps with the host's exp and adds three or more values of a group in an order of its own, so it can choose
+// otherwise between values that are apart by a few units in the last place.
 //
 // Gradient, with u_j = s_{e_j} / D, a_e = scaling dw_j at e = e_j (0 elsewhere), q_e = dscore_e:
 //   ds_e = (a_e - [e chosen, renormalised] sum_j a_j u_j) / D
