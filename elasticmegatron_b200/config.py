@@ -91,7 +91,9 @@ class ModelConfig:
     # RMSNorm of every query and key head before the rotation (Megatron's --qk-layernorm)
     qk_layernorm: bool = False
     # router: softmax after top-k, or (pre_softmax) the softmax over all experts kept as it is, or sigmoid scores divided
-    # by their sum; experts limited to the best group_topk of num_groups groups; weights times topk_scaling_factor
+    # by their sum; experts limited to the best group_topk of num_groups groups; weights times topk_scaling_factor.
+    # A group's value is always a sum of scores.  Megatron sums logits where the softmax comes after top-k, and so may keep
+    # other groups than this router if topk // group_topk > 1; its two other modes agree with this one
     moe_router_score_function: str = "softmax"
     moe_router_pre_softmax: bool = False
     moe_router_num_groups: Optional[int] = None
