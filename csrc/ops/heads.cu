@@ -972,10 +972,16 @@ void pick_stream(const StreamParams& p, int grid, bool inter, bool norm, bool bw
 }
 
 // Dense tensors with 16-byte rows are streamed from a number of heads up, below which the rings' start costs more than the
-// loads that they hide.  Heads of 128, groups of 4 + 2, in L2, direct / streamed: forward 24576 heads 4.7 / 5.6 us, 49152
-// 7.4 / 7.3, 98304 11.8 / 11.2; backward with norm 12288 heads 9.0 / 8.6, 24576 13.2 / 11.5, 49152 19.2 / 14.4 (heads of 64
-// and single-head groups cross at 24576 to 49152 too).  They are streamed at any size where r = 8 mod 16, which
-// the direct kernel would take by single channels.
+// loads that they hide.  Direct / streamed in us, groups of 4 + 2 whole heads of 64 / 128 / 256 / 512 channels, calls back to back:
+//   norm forward   24576 heads  bf16 3.0/3.8  4.4/5.0    7.2/7.4    10.9/10.4   fp32 3.7/4.6  5.9/5.6    9.3/8.7    16.7/17.6
+//                  49152             4.5/4.6  7.1/7.3   11.6/10.8   25.1/21.8        5.5/5.5  9.6/8.4   17.2/17.6   34.4/34.5
+//                  98304             7.2/6.7 11.5/10.5  27.1/22.2   54.2/39.1        9.0/8.2 17.3/17.0  35.4/34.8   66.5/69.8
+//   norm backward  12288             5.2/6.4  7.3/6.8   10.1/9.2    16.6/12.2        5.3/6.6  7.5/8.1   10.6/11.0   18.5/16.2
+//                  24576             7.1/7.1  9.7/9.0   15.7/11.8   25.8/17.9        7.2/7.9 10.5/10.3  16.7/15.5   32.9/30.8
+//                  49152             9.6/9.2 14.8/11.6  24.8/17.5   56.1/33.4       10.4/10.1 16.2/14.7  32.2/30.5   55.2/55.0
+// The rotation alone crosses where the forward does.  Larger calls gain more in 16 bits (196608 heads of 128: 26.9/21.6 and
+// 56.1/32.8) and nothing or less in fp32 (of 512: 131.5/140.6 and 190.7/216.4).  They are streamed at any size where
+// r = 8 mod 16, which the direct kernel would take by single channels.
 bool streams(const HeadParams& p, Access a, const at::Tensor& t, const at::Tensor& other) {
   const long long heads = p.tokens * p.G * p.S, from = other.defined() ? 24576 : 49152;  // (other: the norm's backward)
   return (a.direct ? heads >= from : a.stream) && t.is_contiguous() &&
