@@ -201,11 +201,10 @@ std::vector<at::Tensor> linear_ce_fwd(at::Tensor x, at::Tensor w, at::Tensor lab
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t T = x.size(0), V = w.size(0);
   TORCH_CHECK(V > 0 && col0 >= 0 && col0 + V <= vocab && (raw || V == vocab), "columns outside the vocabulary");
-  // the loss (or the label's logit) has memory of its own: a caller may change it in place while the statistics are kept
-  auto out = new_empty({T}, x, at::kFloat);
-  auto stats = new_empty({raw ? 3 : 2, T}, x, at::kFloat).unbind(0);
-  stats.insert(stats.begin(), out);
-  if (T == 0) return stats;
+  // each has memory of its own: a caller may change the loss in place while the statistics are kept
+  std::vector<at::Tensor> out;
+  for (int i = 0; i < (raw ? 4 : 3); ++i) out.push_back(new_empty({T}, x, at::kFloat));
+  if (T == 0) return out;
   const int64_t tiles = (V + 255) / 256;
   auto part = new_empty({tiles * T * 2 + T}, x, at::kFloat);  // and the labels' logits
   CeArgs ce = ce_args(labels, col0, vocab, ignore);
@@ -213,14 +212,13 @@ std::vector<at::Tensor> linear_ce_fwd(at::Tensor x, at::Tensor w, at::Tensor lab
   ce.target = part.data_ptr<float>() + tiles * T * 2;
   auto xr = tma_rows(x), wr = tma_rows(w);
   linear_ce_gemm(xr, wr, ce, false, at::Tensor());
-  float* o = stats[1].data_ptr<float>();
   launch_early(
       ce_join_kernel, (int)((T + 31) / 32), 1024, 0, ce, reinterpret_cast<const __nv_bfloat16*>(xr.data_ptr()), xr.stride(0),
       reinterpret_cast<const __nv_bfloat16*>(wr.data_ptr()), wr.stride(0), (int)x.size(1), (int)T, (int)tiles, (int)V, raw,
-      out.data_ptr<float>(), o, o + T, raw ? o + 2 * T : nullptr);
+      out[0].data_ptr<float>(), out[1].data_ptr<float>(), out[2].data_ptr<float>(), raw ? out[3].data_ptr<float>() : nullptr);
   EMB_LAUNCH_CHECK();
   count_launch();
-  return stats;
+  return out;
 }
 
 // {dx [T, H] bf16, dw [V, H] bf16}, each undefined where it is not wanted; with `dw_accum` (fp32 [V, H]) the weight
@@ -265,11 +263,9 @@ std::vector<at::Tensor> linear_ce_bwd(at::Tensor dloss, at::Tensor x, at::Tensor
   ce.dloss = g.data_ptr<float>();
   // dx of few rows and dw of few words have few output tiles and a long sum: it is split, fp32 parts joined in order
   // (dx of 512 x 129024 x 4096: 572 -> 436 us, dw of 8192 x 1000 x 512: 82 -> 26 us against whole sums on single SMs).
-  // The parts of a product fill the SMs once (a 128 x 256 tile each) and are joined before the next product.  A piece that
-  // would be one part is added to the sum by the product itself.
+  // The parts of a product fill the SMs once (a 128 x 256 tile each) and are joined before the next product.
   const Split sx(rows, H), sw(std::min(piece, V), H);
-  const bool split = want_dx && (rows > T || ((sx.pair ? sx.tiles : sx.tiles * 2) <= sx.slots &&
-                                              (pieces == 1 || sx.shares(piece) > 1)));
+  const bool split = want_dx && (rows > T || (sx.pair ? sx.tiles : sx.tiles * 2) <= sx.slots);
   const bool split_w = wants_w && pieces == 1 && sw.shares(xs.size(0)) > 1;
   at::Tensor total;  // dx over several pieces
   if (want_dx && pieces > 1) {
