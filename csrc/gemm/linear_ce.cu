@@ -14,8 +14,8 @@
 // the square root of two of what rounding the result alone costs (relative error 0.0024 against 0.00166 at 129 to 8000
 // tokens and 1000 to 32000 words; the output layer with kept bf16 logits: 0.0024 to 0.0026).  Up to 128 rows P is kept as two
 // bf16 rows, P and its rounding error, and the error is that of the result alone: the epilogue of the single-SM product, a
-// tile of 128 rows, writes both, and reading w bounds the backward (weights of 129024 x 4096, 65 / 128 rows: 790 / 842 us; with
-// one row each 733 / 732).  With more rows the tensor cores bound it, and 10 T V H instead of 6 would cost in proportion.
+// tile of 128 rows, writes both, and reading w bounds the backward (weights of 129024 x 4096, 65 / 128 rows: 790 to 870 / 840
+// to 960 us by run; with one row each 730 / 730 to 810).  With more rows the tensor cores bound it, and 10 T V H instead of 6 would cost in proportion.
 #include "linear_ce.cuh"
 
 #include <c10/cuda/CUDAGuard.h>
